@@ -126,13 +126,14 @@ def prepare(case, seed):
         pages = [-(-h // P) for h in held]
         tokens = sum(max(n, 0) for n in new)
         s["max_tokens"] = -(-max(tokens, 1) // 64) * 64  # the step's token buffers are padded
-        free = sum(-(-(h + max(n, 0)) // P) - p for h, n, p in zip(held, new, pages)) + 5
-        ids = torch.randperm(sum(pages) + free, generator=gen, device="cuda", dtype=torch.int32)
+        free = min(sum(-(-(h + max(n, 0)) // P) - p for h, n, p in zip(held, new, pages)) + 5, case["B"] * case["width"] + 5 - sum(pages))
+        pool = case["B"] * case["width"] + 5
+        ids = torch.randperm(pool, generator=gen, device="cuda", dtype=torch.int32)
         table = torch.full((case["B"], case["width"]), -1, dtype=torch.int32, device="cuda")
         mask = torch.arange(case["width"], device="cuda")[None] < _ints(pages)[:, None]
         table[mask] = ids[: sum(pages)]
-        s["free_pages"] = torch.full((ids.numel(),), -1, dtype=torch.int32, device="cuda")
-        s["free_pages"][:free] = ids[sum(pages):]
+        s["free_pages"] = torch.full((pool,), -1, dtype=torch.int32, device="cuda")
+        s["free_pages"][:free] = ids[sum(pages): sum(pages) + free]
         s |= {"k_len": _ints(held), "n_new": _ints(new), "block_table": table, "free_count": _ints([free])}
         s["tables"] = {"q_start": table.new_empty(case["B"] + 1), "k_len": table.new_empty(case["B"]),
                        "slots": table.new_empty(s["max_tokens"]), "counts": table.new_empty(2)}  # where the step's tables go
@@ -200,11 +201,13 @@ def run(s):
         if s["op"] == "plan":
             p = fa.cache_plan(s["k_len"], s["n_new"], s["block_table"], s["free_pages"], s["free_count"], s["P"],
                               out=fa.CachePlan(**s["tables"]))
-            return {"q_start": p.q_start, "k_len": p.k_len, "slots": p.slots, "counts": p.counts, "block_table": s["block_table"]}
+            return {"q_start": p.q_start, "k_len": p.k_len, "slots": p.slots, "counts": p.counts,
+                    "block_table": s["block_table"], "free_pages": s["free_pages"]}
+        cache = s.get("cache") or s.setdefault("cache", fa.PagedCache(s["k_cache"], s["v_cache"]))  # a program has one for good
         if s["op"] == "write":
-            fa.cache_write(s["k"], s["v"], s["k_cache"], s["v_cache"], s["slots"])
+            fa.cache_write(s["k"], s["v"], cache, s["slots"])
             return {"k_cache": s["k_cache"], "v_cache": s["v_cache"]}
-        return fa.attention_shared_prefix(s["q"], s["k_cache"], s["v_cache"], s["q_start"], s["k_len"], s["block_table"],
+        return fa.attention_shared_prefix(s["q"], cache, s["q_start"], s["k_len"], s["block_table"],
                                           prefix_table=s["prefix_table"], prefix_len=s["prefix"], out=s["out"])
     return {"plan": _plan, "write": _write, "attend": _attend}[s["op"]](s)
 
@@ -238,7 +241,7 @@ def _plan(s):
     slots = torch.where((t < q_start[-1]) & fits[b], slot, -1)
     counts = torch.stack([top - taken, (~fits).sum()])
     return {"q_start": q_start.int(), "k_len": torch.where(fits, k + n, k).int(), "slots": slots.int(), "counts": counts.int(),
-            "block_table": table}
+            "block_table": table, "free_pages": s["free_pages"]}
 
 
 def _write(s):
@@ -295,6 +298,7 @@ def exact(case, seed):
         after, slots, start, refused = [], [], [0], 0
         for b, (h, n) in enumerate(zip(held, new)):
             stack += table[b][-(-(h + n) // P): -(-h // P)]
+        pages = stack + s["free_pages"].tolist()[len(stack):]  # what lies above the count stays where it was
         for b, (h, n) in enumerate(zip(held, new)):
             need = max(0, -(-(h + n) // P) - -(-h // P))
             ok = need <= len(stack) and (not refused or need == 0)
@@ -306,7 +310,7 @@ def exact(case, seed):
             after.append(h + n if ok else h)
         slots += [-1] * (s["max_tokens"] - len(slots))
         return {"q_start": _ints(start), "k_len": _ints(after), "slots": _ints(slots), "counts": _ints([len(stack), refused]),
-                "block_table": _ints(table)}
+                "block_table": _ints(table), "free_pages": _ints(pages)}
     if case["op"] == "write":
         got = {}
         t = (s["slots"] >= 0).nonzero()[:, 0]
