@@ -12,7 +12,9 @@ if the shared library is missing or a call fails, an exception is raised.
 from __future__ import annotations
 
 import ctypes as ct
+import functools
 import os
+from typing import NamedTuple
 
 import numpy as np
 
@@ -49,6 +51,10 @@ EXPORTED_SYMBOLS = (
     "fa_set_reserved_cus",
     "fa_get_reserved_cus",
     "fa_debug_reload_env",
+    "fa_cache_plan",
+    "fa_cache_write",
+    "fa_forward_shared_prefix",
+    "fa_shared_prefix_workspace",
 )
 
 _lib = None
@@ -56,6 +62,11 @@ _lib = None
 
 class FlashAttentionError(RuntimeError):
     pass
+
+
+class _PagedCacheStruct(ct.Structure):  # fa_paged_cache
+    _fields_ = [("k", ct.c_void_p), ("v", ct.c_void_p), ("k_strides", ct.c_int64 * 3), ("v_strides", ct.c_int64 * 3),
+                ("n_pages", ct.c_int), ("page_size", ct.c_int), ("heads", ct.c_int), ("head_dim", ct.c_int)]
 
 
 def lib() -> ct.CDLL:
@@ -139,6 +150,16 @@ def bind(path: str) -> ct.CDLL:
     L.fa_get_reserved_cus.restype = ct.c_int
     L.fa_debug_reload_env.argtypes = []
     L.fa_debug_reload_env.restype = None
+    vp, i, i64 = ct.c_void_p, ct.c_int, ct.c_int64
+    L.fa_cache_plan.argtypes = [vp, vp, vp, i64, vp, vp, vp, vp, vp, vp, i, i, i, i, i, vp, FloatPtr]
+    L.fa_cache_plan.restype = i
+    L.fa_cache_write.argtypes = [vp, vp, i64, i64, i64, i64, ct.POINTER(_PagedCacheStruct), vp, i, vp, FloatPtr]
+    L.fa_cache_write.restype = i
+    L.fa_forward_shared_prefix.argtypes = [vp, i64, i64, vp, i64, i64, ct.POINTER(_PagedCacheStruct), vp, i, vp, i64, i, vp, vp,
+                                           i, i, i, i, i, ct.c_float, i, vp, ct.c_size_t, vp, FloatPtr]
+    L.fa_forward_shared_prefix.restype = i
+    L.fa_shared_prefix_workspace.argtypes = [i] * 7
+    L.fa_shared_prefix_workspace.restype = ct.c_size_t
     return L
 
 
@@ -392,6 +413,184 @@ def attention_block_general(q, k_blk, v_blk, state: BlockState, last: bool, caus
     _check(rc)
     state.first = False
     return out
+
+
+class PagedCache:
+    """A paged K/V cache (``fa_paged_cache``): ``k`` and ``v`` are float16 or bfloat16 GPU tensors of one shape
+    [n_pages, Hkv, page_size, D], with any strides of the first three axes (token-major pages are a permuted view, K and V
+    in one pool are slices of it).  page_size a power of two from 16 to 65536, D of 64, 128 or 256.  The tensors are held, not copied."""
+
+    def __init__(self, k, v):
+        import torch
+
+        for t in (k, v):
+            if not t.is_cuda or t.dtype not in (torch.float16, torch.bfloat16) or t.dim() != 4 or t.stride(3) != 1:
+                raise ValueError("k, v must be float16 or bfloat16 GPU tensors [n_pages, Hkv, page_size, D] whose rows are contiguous")
+        if v.shape != k.shape or v.dtype != k.dtype or v.device != k.device:
+            raise ValueError("k and v must share shape, dtype and device")
+        self.k, self.v, self.dtype, self.device, self.device_index = k, v, k.dtype, k.device, k.device.index
+        self.n_pages, self.heads, self.page_size, self.head_dim = k.shape
+        self.c = _PagedCacheStruct(k.data_ptr(), v.data_ptr(), (ct.c_int64 * 3)(*k.stride()[:3]), (ct.c_int64 * 3)(*v.stride()[:3]),
+                                   self.n_pages, self.page_size, self.heads, self.head_dim)
+        self.ref = ct.byref(self.c)
+        self.dtype_code = 0 if k.dtype == torch.float16 else 1
+
+
+class CachePlan(NamedTuple):
+    """Tables of one serving step, int32 GPU tensors: ``q_start`` [B + 1], ``k_len`` [B], ``slots`` [max_tokens], ``counts``
+    [2] (free pages left, requests refused).  ``k_len`` and ``counts[:1]`` are the next step's ``k_len`` and ``free_count``;
+    a program keeps two of these and alternates."""
+
+    q_start: object
+    k_len: object
+    slots: object
+    counts: object
+
+
+def make_cache_plan(B: int, max_tokens: int, device) -> CachePlan:
+    """A ``CachePlan``'s tensors for ``B`` requests and up to ``max_tokens`` new tokens a step."""
+    import torch
+
+    return CachePlan(*(torch.empty(n, dtype=torch.int32, device=device) for n in (B + 1, B, max_tokens, 2)))
+
+
+def _on_device(index: int):
+    """The current device for a launch on GPU ``index``: nothing to do when it is that already."""
+    import contextlib
+
+    import torch
+
+    return contextlib.nullcontext() if torch.cuda.current_device() == index else torch.cuda.device(index)
+
+
+def _int_tensor(t, name: str, index: int, n: int) -> int:
+    """Address of a contiguous int32 tensor of ``n`` entries on GPU ``index``."""
+    import torch
+
+    if t.dtype != torch.int32 or t.get_device() != index or t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor of {n} entries on the call's GPU")
+    return t.data_ptr()
+
+
+def _table(t, name: str, index: int, rows: int):
+    import torch
+
+    if t.dim() != 2 or t.dtype != torch.int32 or t.get_device() != index or t.shape[0] != rows or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError(f"{name} must be an int32 tensor [{rows}, width] with contiguous rows on the call's GPU")
+    return t.data_ptr(), max(t.stride(0), t.shape[1]) if rows == 1 else t.stride(0), t.shape[1]
+
+
+def cache_plan(k_len, n_new, block_table, free_pages, free_count, page_size: int, max_tokens: int = None, out: CachePlan = None,
+               stream=None, timed: bool = False):
+    """``fa_cache_plan``: block table, slot map and lengths of one serving step, on the GPU.  ``k_len``, ``n_new`` [B] keys
+    each request holds and adds (negative: drops from its end); ``block_table`` [B, width] and the stack ``free_pages`` are
+    updated in place, ``free_count`` [1] counts its pages.  All int32 GPU tensors.  Returns a ``CachePlan`` (``out``, or a
+    new one for ``max_tokens`` tokens); a refused request keeps its ``k_len``."""
+    import torch
+
+    B, dev = k_len.numel(), k_len.get_device()
+    if dev < 0:
+        raise FlashAttentionError("cache_plan() needs GPU tensors; there is no CPU fallback")
+    if out is None:
+        if max_tokens is None:
+            raise ValueError("cache_plan() needs max_tokens or out")
+        out = make_cache_plan(B, max_tokens, k_len.device)
+    elif max_tokens is not None and max_tokens != out.slots.numel():
+        raise ValueError("max_tokens must be the size of out.slots")
+    if stream is None:
+        stream = torch.cuda.current_stream(dev)
+    table, stride, width = _table(block_table, "block_table", dev, B)
+    max_tokens, cap = out.slots.numel(), free_pages.numel()
+    ms = ct.c_float(0.0)
+    with _on_device(dev):
+        _check(lib().fa_cache_plan(
+            _int_tensor(k_len, "k_len", dev, B), _int_tensor(n_new, "n_new", dev, B), table, stride,
+            _int_tensor(free_pages, "free_pages", dev, cap), _int_tensor(free_count, "free_count", dev, 1),
+            _int_tensor(out.q_start, "out.q_start", dev, B + 1), _int_tensor(out.k_len, "out.k_len", dev, B),
+            _int_tensor(out.slots, "out.slots", dev, max_tokens), _int_tensor(out.counts, "out.counts", dev, 2),
+            B, width, page_size, cap, max_tokens, _stream_handle(stream), ct.byref(ms) if timed else None))
+    return (out, float(ms.value)) if timed else out
+
+
+def _token_rows(t, name: str, heads, cache: "PagedCache"):
+    if t.dim() != 3 or t.dtype != cache.dtype or t.get_device() != cache.device_index or t.shape[2] != cache.head_dim or \
+            (heads is not None and t.shape[1] != heads) or (t.stride(2) != 1 and t.numel()):
+        raise ValueError(f"{name} must be [T, heads, {cache.head_dim}] with contiguous rows, of the cache's dtype and GPU")
+    return t.data_ptr(), t.stride(0), t.stride(1)
+
+
+def cache_write(k, v, cache: PagedCache, slots, stream=None, timed: bool = False):
+    """``fa_cache_write``: row t of ``k`` and ``v`` [T, Hkv, D] (any token and head strides) goes into slot ``slots[t]`` of the
+    cache (int32, a ``CachePlan``'s); negative slots and slots on no page of the cache are skipped."""
+    import torch
+
+    T, dev = k.shape[0], cache.device_index
+    if v.shape != k.shape:
+        raise ValueError("k and v must share one [T, Hkv, D] shape")
+    if slots.numel() < T:
+        raise ValueError("slots must name a slot for every token")
+    kp, kt, kh = _token_rows(k, "k", cache.heads, cache)
+    vp, vt, vh = _token_rows(v, "v", cache.heads, cache)
+    if stream is None:
+        stream = torch.cuda.current_stream(dev)
+    ms = ct.c_float(0.0)
+    with _on_device(dev):
+        _check(lib().fa_cache_write(kp, vp, kt, kh, vt, vh, cache.ref, _int_tensor(slots, "slots", dev, slots.numel()), T,
+                                    _stream_handle(stream), ct.byref(ms) if timed else None))
+    return float(ms.value) if timed else None
+
+
+@functools.lru_cache(maxsize=4096)
+def _shared_prefix_workspace(device: int, *sizes) -> int:
+    return lib().fa_shared_prefix_workspace(*sizes)
+
+
+def attention_shared_prefix(q, cache: PagedCache, q_start, k_len, block_table, prefix_table=None, prefix_len: int = 0,
+                            causal: bool = True, scale: float = None, max_k_len: int = None, out=None, stream=None,
+                            timed: bool = False):
+    """``fa_forward_shared_prefix``: attention of a batch of requests behind one shared prefix.  ``q`` [T, Hq, D] packed new
+    tokens (any token and head strides; Hq a multiple of the cache's heads), request b's being rows ``q_start[b]`` to
+    ``q_start[b + 1]``; they see the ``prefix_len`` keys on the pages of ``prefix_table`` and the request's own ``k_len[b]``
+    keys on the pages of ``block_table[b]``, the new tokens' own among them (already written), with ``causal`` only up to their
+    own.  ``max_k_len``: a bound on ``k_len`` that the launch is divided for (default: what the table names).  Rows of
+    ``out`` that belong to no request are left as they are (0 in a new one).  Returns ``out`` (and the kernel-only
+    milliseconds when ``timed``)."""
+    import torch
+
+    dev = cache.device_index
+    qp, qt, qh = _token_rows(q, "q", None, cache)
+    T, Hq, D = q.shape
+    if out is None:
+        out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape:
+        raise ValueError("out must have q's shape")
+    op, ot, oh = _token_rows(out, "out", Hq, cache)
+    B = k_len.numel()
+    if Hq % cache.heads:
+        raise ValueError("q's heads must be a multiple of the cache's")
+    table, stride, width = _table(block_table, "block_table", dev, B)
+    if prefix_len:
+        if prefix_table is None or prefix_table.numel() * cache.page_size < prefix_len:
+            raise ValueError("prefix_table must name the pages of prefix_len keys")
+        prefix = _int_tensor(prefix_table, "prefix_table", dev, prefix_table.numel())
+    else:
+        prefix = None
+    room = width * cache.page_size
+    max_k = room if max_k_len is None else max(0, min(max_k_len, room))
+    if stream is None:
+        stream = torch.cuda.current_stream(dev)
+    n = _shared_prefix_workspace(dev, T, B, Hq, cache.heads, D, prefix_len, max_k)
+    ms = ct.c_float(0.0)
+    with _on_device(dev):
+        workspace = torch.empty(n, dtype=torch.uint8, device=q.device)
+        if isinstance(stream, int) or stream != torch.cuda.current_stream(dev):
+            workspace.record_stream(torch.cuda.ExternalStream(stream) if isinstance(stream, int) else stream)
+        _check(lib().fa_forward_shared_prefix(
+            qp, qt, qh, op, ot, oh, cache.ref, prefix, prefix_len, table, stride, width, _int_tensor(q_start, "q_start", dev, B + 1),
+            _int_tensor(k_len, "k_len", dev, B), T, B, Hq, cache.dtype_code, FLAG_CAUSAL if causal else 0,
+            D ** -0.5 if scale is None else scale, max_k, workspace.data_ptr(), n, _stream_handle(stream),
+            ct.byref(ms) if timed else None))
+    return (out, float(ms.value)) if timed else out
 
 
 def init_half(t, seed: int, stream=None) -> None:

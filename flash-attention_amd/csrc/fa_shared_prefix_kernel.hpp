@@ -1,0 +1,364 @@
+// Attention of a batch whose requests share a long prefix, over a paged K/V cache.  Row (t, h), token t of request b and
+// query head h of K/V head h / g:
+//     O = sum_j p_j V_j / sum_j p_j,   p_j = exp(scale Q.K_j),   j over the Lp keys of the prefix and over the request's
+//     own keys j <= k_len[b] - n[b] + (t - q_start[b])  (causal; all k_len[b] of them otherwise).
+// The sum over j falls into parts that are computed apart and joined by their maxima (log-sum-exp): the prefix part is one
+// matrix product for the whole batch, its rows being the g heads of ALL tokens stacked up against each K/V head, so the
+// prefix is read from memory once per 128 stacked rows instead of once per request; the own part has the rows of one
+// request.  Both parts are divided over ranges of keys until the chip is full.
+// A workgroup has 4 waves of 32 rows and walks its range in tiles of kTk keys (transposed scores S^T = K.Q^T, the score
+// registers rounded to 16 bits as B operand of O^T += V^T.P^T, swizzled LDS tiles: the lane geometry of
+// fa_fwd_general_kernel.hpp).  fa_shared_prefix_merge_kernel joins the parts.
+//
+// Masks.  A tile that holds a masked place for some row of the wave (the end of the range, the causal diagonal, a page that
+// is none) takes the masked form of the step: scores of masked places become -inf whatever K holds there, and V is
+// multiplied with its infinities and NaN taken out (0 x NaN is NaN), which are then added to the rows that do see them.
+// Rows that see no key give 0.
+#pragma once
+#include "fa_fwd_general_kernel.hpp"
+#include "fa_paged_index.hpp"
+
+namespace fa {
+
+struct SharedPrefixParams {
+    const uint16_t* q;
+    uint16_t* o;
+    const uint16_t* kc;
+    const uint16_t* vc;
+    int64_t q_tok, q_head, o_tok, o_head;
+    CacheStrides ks, vs;
+    const int* prefix_table;
+    const int* block_table;
+    int64_t table_stride;
+    const int* q_start;
+    const int* k_len;
+    float* part_o;   // [parts][T * Hq][D], un-normalised
+    float* part_ml;  // [parts][T * Hq][2]: largest score (log2 units) and sum of exp2(score - largest)
+    int T, B, Hkv, g, log2_page, n_pages, prefix_len, table_width, causal;
+    float scale_log2e;
+    int prefix_parts, prefix_range;  // key ranges of the prefix, keys per range (whole tiles)
+    int own_parts, own_range;        // the same for the requests' own keys; the last range takes whatever is left
+    int prefix_blocks;               // workgroups of the prefix part: the first ones of the grid
+};
+
+template <typename E>
+struct Elem;
+template <>
+struct Elem<_Float16> {
+    typedef _Float16 v8 __attribute__((ext_vector_type(8)));
+    typedef _Float16 v4 __attribute__((ext_vector_type(4)));
+    static constexpr unsigned kExpMask = 0x7c00;
+    static __device__ __forceinline__ f32x16 mfma(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+};
+template <>
+struct Elem<__bf16> {
+    typedef __bf16 v8 __attribute__((ext_vector_type(8)));
+    typedef __bf16 v4 __attribute__((ext_vector_type(4)));
+    static constexpr unsigned kExpMask = 0x7f80;
+    static __device__ __forceinline__ f32x16 mfma(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+};
+
+// max that keeps NaN (v_maximum3_f32): a row that sees a NaN score is NaN, and no operand is canonicalised first.
+__device__ __forceinline__ float max_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
+// Infinities and NaN of a V fragment: taken out (returned fragment), and their places (kind 1 NaN, 2 +inf, 3 -inf) as ones.
+template <typename E>
+__device__ __forceinline__ typename Elem<E>::v8 finite_part(typename Elem<E>::v8 x, bool& special) {
+    u32x4 u = __builtin_bit_cast(u32x4, x);
+    constexpr unsigned m = Elem<E>::kExpMask;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if ((u[i] & m) == m) u[i] &= 0xffff0000u, special = true;
+        if ((u[i] & (m << 16)) == m << 16) u[i] &= 0x0000ffffu, special = true;
+    }
+    return __builtin_bit_cast(typename Elem<E>::v8, u);
+}
+template <typename E>
+__device__ __forceinline__ typename Elem<E>::v8 special_part(typename Elem<E>::v8 x, int kind) {
+    const u32x4 u = __builtin_bit_cast(u32x4, x);
+    constexpr unsigned m = Elem<E>::kExpMask;
+    typename Elem<E>::v8 r;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const unsigned h = (u[i / 2] >> (16 * (i & 1))) & 0xffffu, a = h & 0x7fffu;
+        const int k = a > m ? 1 : a < m ? 0 : h == a ? 2 : 3;
+        r[i] = (E)(k == kind ? 1.0f : 0.0f);
+    }
+    return r;
+}
+
+template <int D>
+struct SharedCfg {
+    static constexpr int kTk = 64;
+    static constexpr int kOcc = D == 256 ? 1 : 2;
+};
+
+template <typename E, int D>
+__global__ __launch_bounds__(256, SharedCfg<D>::kOcc) void fa_shared_prefix_kernel(const SharedPrefixParams p) {
+    using HD = HeadDim<D>;
+    using v8 = typename Elem<E>::v8;
+    constexpr int TK = SharedCfg<D>::kTk, KB = TK / 32, kTile = TK * HD::kRow;
+    constexpr int CHUNKS = kTile / 16 / 256, RSTEP = 256 / HD::kChunks;
+    __shared__ __attribute__((aligned(16))) char smem[4 * kTile];
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const LaneGeomD<D> geo = make_lane_geom_d<D>(lane);
+    const int P1 = (1 << p.log2_page) - 1;
+
+    // ---- which rows against which keys
+    const bool own = (int)blockIdx.x >= p.prefix_blocks;
+    int tile, head, part;
+    int row0, rows;              // stacked rows of this tile's request (or of the whole batch), and how many
+    int tok0 = 0, n_tok, keys, key0, key1;
+    const int* table;
+    int table_n;
+    {
+        const int parts = own ? p.own_parts : p.prefix_parts;
+        int x = (int)blockIdx.x - (own ? p.prefix_blocks : 0);
+        part = x % parts;
+        x /= parts;
+        head = x % p.Hkv;
+        tile = x / p.Hkv;
+        if (own) {
+            int lo = 0, hi = p.B;
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (first_row_tile(clamp_int(p.q_start[mid], 0, p.T), mid, p.g, 7) <= tile)
+                    lo = mid;
+                else
+                    hi = mid;
+            }
+            tok0 = clamp_int(p.q_start[lo], 0, p.T);
+            n_tok = clamp_int(p.q_start[lo + 1], tok0, p.T) - tok0;
+            tile -= first_row_tile(tok0, lo, p.g, 7);
+            table = p.block_table + lo * p.table_stride;
+            table_n = p.table_width;
+            const int64_t room = (int64_t)p.table_width << p.log2_page;
+            keys = clamp_int(p.k_len[lo], 0, (int)room);
+            key0 = (int)min((int64_t)part * p.own_range, (int64_t)keys);
+            key1 = part == p.own_parts - 1 ? keys : (int)min((int64_t)key0 + p.own_range, (int64_t)keys);
+        } else {
+            n_tok = clamp_int(p.q_start[p.B], 0, p.T);
+            table = p.prefix_table;
+            table_n = pages_for(p.prefix_len, p.log2_page);
+            keys = p.prefix_len;
+            key0 = part * p.prefix_range;
+            key1 = min(key0 + p.prefix_range, keys);
+        }
+        row0 = tile * 128;
+        rows = n_tok * p.g;
+        if (tile < 0 || row0 >= rows) return;
+    }
+    const bool causal = own && p.causal != 0;
+    const int part_all = own ? p.prefix_parts + part : part;
+    const int R = min(row0 + wave * 32 + geo.r, rows - 1);  // this lane's row; past the end the last one, not stored
+    const bool valid = row0 + wave * 32 + geo.r < rows;
+    const bool wave_valid = row0 + wave * 32 < rows;
+    const int ti = R / p.g, tok = tok0 + ti, hq = head * p.g + (R - ti * p.g);
+    const int Hq = p.Hkv * p.g;
+    const int64_t slot = (int64_t)part_all * p.T * Hq + (int64_t)tok * Hq + hq;
+    // the last key this row sees; a workgroup need not walk past its last row's
+    const int limit = causal ? min(keys - 1, keys - n_tok + ti) : keys - 1;
+    if (causal) {
+        const int last_ti = (min(row0 + 128, rows) - 1) / p.g;
+        key1 = min(key1, keys - n_tok + last_ti + 1);
+    }
+    const int n_tiles = key1 > key0 ? (key1 - key0 + TK - 1) / TK : 0;
+
+    v8 qf[HD::kSteps];
+    {
+        const uint16_t* qr = p.q + tok * p.q_tok + hq * p.q_head + geo.hh * 8;
+#pragma unroll
+        for (int ks = 0; ks < HD::kSteps; ++ks) qf[ks] = *reinterpret_cast<const v8*>(qr + ks * 16);
+    }
+
+    f32x16 oacc[HD::kBlocks];
+    float m_run = -1e30f, l_run = 0.0f;
+#pragma unroll
+    for (int db = 0; db < HD::kBlocks; ++db)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) oacc[db][e] = 0.0f;
+
+    const int st_row = tid / HD::kChunks, st_ch = tid % HD::kChunks;
+    u32x4 st_k[CHUNKS], st_v[CHUNKS];
+    // the page of a key, -1 where there is none; a row on no page is fetched from page 0: its score is masked
+    auto page_of = [&](int key) -> int {
+        const int j = key >> p.log2_page;
+        const int page = j < table_n ? table[j] : -1;
+        return page_ok(page, p.n_pages) ? page : -1;
+    };
+    auto stage_load = [&](int t) {
+#pragma unroll
+        for (int i = 0; i < CHUNKS; ++i) {
+            const int key = key0 + t * TK + st_row + i * RSTEP, page = max(page_of(key), 0);
+            st_k[i] = *reinterpret_cast<const u32x4*>(p.kc + cache_offset(p.ks, page, head, key & P1) + st_ch * 8);
+            st_v[i] = *reinterpret_cast<const u32x4*>(p.vc + cache_offset(p.vs, page, head, key & P1) + st_ch * 8);
+        }
+    };
+    auto stage_write = [&](int buf) {
+        char* kw = smem + buf * 2 * kTile;
+#pragma unroll
+        for (int i = 0; i < CHUNKS; ++i) {
+            const int row = st_row + i * RSTEP;
+            *reinterpret_cast<u32x4*>(kw + row * HD::kRow + ((st_ch ^ (row & HD::kKMask)) << 4)) = st_k[i];
+            *reinterpret_cast<u32x4*>(kw + kTile + row * HD::kRow + ((st_ch ^ ((row & HD::kVMask) << 2)) << 4)) = st_v[i];
+        }
+    };
+    auto v_frag = [&](const char* vb, int kk, int db) -> v8 {
+        const char* a0 = vb + geo.v_rd[db] + kk * 16 * HD::kRow;
+        const short4_t t0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t*)(a0));
+        const short4_t t1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t*)(a0 + 8 * HD::kRow));
+        return __builtin_bit_cast(v8, __builtin_shufflevector(t0, t1, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+
+    if (n_tiles > 0) {
+        stage_load(0);
+        stage_write(0);
+    }
+    __syncthreads();
+    for (int t = 0; t < n_tiles; ++t) {
+        if (t + 1 < n_tiles) stage_load(t + 1);
+        if (wave_valid) {
+            const char* kb = smem + (t & 1) * 2 * kTile;
+            const char* vb = kb + kTile;
+            const int first = key0 + t * TK;
+            f32x16 s[KB];
+#pragma unroll
+            for (int b = 0; b < KB; ++b) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[b][e] = 0.0f;
+#pragma unroll
+                for (int ks = 0; ks < HD::kSteps; ++ks)
+                    s[b] = Elem<E>::mfma(*reinterpret_cast<const v8*>(kb + geo.k_rd[ks] + b * 32 * HD::kRow), qf[ks], s[b]);
+            }
+            // which 16-key groups of the tile lie on a page
+            unsigned groups = 0;
+#pragma unroll
+            for (int c = 0; c < TK / 16; ++c) groups |= page_of(first + 16 * c) >= 0 ? 1u << c : 0u;
+            const int lim = min(limit, key1 - 1) - first;
+            const bool masked = __any(lim < TK - 1) || groups != (1u << (TK / 16)) - 1;
+            if (masked) {
+#pragma unroll
+                for (int b = 0; b < KB; ++b)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const int k = 32 * b + 8 * (e >> 2) + (e & 3);
+                        if (k + 4 * geo.hh > lim || !((groups >> (k >> 4)) & 1)) s[b][e] = -__builtin_inff();
+                    }
+            }
+            float mx = s[0][0];
+#pragma unroll
+            for (int b = 0; b < KB; ++b)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) mx = max_nan(mx, s[b][e]);
+            {
+                float a, b;
+                half_wave_pair(mx, a, b);
+                mx = max_nan(a, b) * p.scale_log2e;
+            }
+            if (!__all(mx - m_run <= kRescaleSlack)) {
+                const float m_new = max_nan(m_run, mx), alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+                m_run = m_new;
+                l_run *= alpha;
+#pragma unroll
+                for (int db = 0; db < HD::kBlocks; ++db)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) oacc[db][e] *= alpha;
+            }
+            v8 pf[2 * KB];
+#pragma unroll
+            for (int b = 0; b < KB; ++b)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][e], p.scale_log2e, -m_run));
+                    l_run += x;
+                    pf[2 * b + e / 8][e % 8] = (E)x;
+                }
+            if (!masked) {
+#pragma unroll
+                for (int kk = 0; kk < 2 * KB; ++kk)
+#pragma unroll
+                    for (int db = 0; db < HD::kBlocks; ++db) oacc[db] = Elem<E>::mfma(v_frag(vb, kk, db), pf[kk], oacc[db]);
+            } else {
+                bool special = false;
+#pragma unroll
+                for (int kk = 0; kk < 2 * KB; ++kk)
+#pragma unroll
+                    for (int db = 0; db < HD::kBlocks; ++db)
+                        oacc[db] = Elem<E>::mfma(finite_part<E>(v_frag(vb, kk, db), special), pf[kk], oacc[db]);
+                if (__any(special)) {
+                    v8 sees[2 * KB];  // 1 where the row sees the key
+#pragma unroll
+                    for (int kk = 0; kk < 2 * KB; ++kk)
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const int k = 16 * kk + 8 * (i >> 2) + (i & 3);
+                            sees[kk][i] = (E)(k + 4 * geo.hh <= lim && ((groups >> (k >> 4)) & 1) ? 1.0f : 0.0f);
+                        }
+                    for (int kind = 1; kind <= 3; ++kind) {
+                        const unsigned bits = kind == 1 ? 0x7fc00000u : kind == 2 ? 0x7f800000u : 0xff800000u;
+#pragma unroll
+                        for (int db = 0; db < HD::kBlocks; ++db) {
+                            f32x16 n;
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) n[e] = 0.0f;
+#pragma unroll
+                            for (int kk = 0; kk < 2 * KB; ++kk)
+                                n = Elem<E>::mfma(special_part<E>(v_frag(vb, kk, db), kind), sees[kk], n);
+#pragma unroll
+                            for (int e = 0; e < 16; ++e)
+                                if (n[e] > 0.0f) oacc[db][e] += __builtin_bit_cast(float, bits);
+                        }
+                    }
+                }
+            }
+        }
+        if (t + 1 < n_tiles) stage_write((t + 1) & 1);
+        __syncthreads();
+    }
+
+    if (!valid) return;
+    float l0, l1;
+    half_wave_pair(l_run, l0, l1);
+    if (geo.hh == 0) {
+        p.part_ml[2 * slot] = m_run;
+        p.part_ml[2 * slot + 1] = l0 + l1;
+    }
+    float* oa = p.part_o + slot * D;
+#pragma unroll
+    for (int db = 0; db < HD::kBlocks; ++db)
+#pragma unroll
+        for (int g4 = 0; g4 < 4; ++g4) {
+            const f32x4 x = {oacc[db][4 * g4], oacc[db][4 * g4 + 1], oacc[db][4 * g4 + 2], oacc[db][4 * g4 + 3]};
+            *reinterpret_cast<f32x4*>(oa + 32 * db + 8 * g4 + 4 * geo.hh) = x;
+        }
+}
+
+// O = sum_s w_s o_s / sum_s w_s l_s,  w_s = exp2(m_s - max_s m_s): D / 4 lanes per row, rows of no request left alone.
+template <typename E, int D>
+__global__ __launch_bounds__(256) void fa_shared_prefix_merge_kernel(const SharedPrefixParams p) {
+    constexpr int LPR = D / 4, RPB = 256 / LPR;
+    const int c = threadIdx.x % LPR, Hq = p.Hkv * p.g, parts = p.prefix_parts + p.own_parts;
+    const int64_t rows = (int64_t)p.T * Hq, i = (int64_t)blockIdx.x * RPB + threadIdx.x / LPR;
+    if (i >= rows) return;
+    const int tok = (int)(i / Hq), hq = (int)(i - (int64_t)tok * Hq);
+    if (tok < clamp_int(p.q_start[0], 0, p.T) || tok >= clamp_int(p.q_start[p.B], 0, p.T)) return;
+    float m = -1e30f;
+    for (int s = 0; s < parts; ++s) m = max_nan(m, p.part_ml[2 * (s * rows + i)]);
+    f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    float l = 0.0f;
+    for (int s = 0; s < parts; ++s) {
+        const int64_t r = s * rows + i;
+        const float w = __builtin_amdgcn_exp2f(p.part_ml[2 * r] - m), ls = p.part_ml[2 * r + 1];
+        if (ls == 0.0f) continue;
+        l += w * ls;
+        acc += *reinterpret_cast<const f32x4*>(p.part_o + r * D + 4 * c) * w;
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    typename Elem<E>::v4 out;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) out[e] = (E)(acc[e] * inv);
+    *reinterpret_cast<typename Elem<E>::v4*>(p.o + tok * p.o_tok + hq * p.o_head + 4 * c) = out;
+}
+
+}  // namespace fa

@@ -25,6 +25,7 @@
 #include "fa_fwd_w64_kernel.hpp"
 #include "fa_fwd_general_kernel.hpp"
 #include "fa_fwd_hd_kernel.hpp"
+#include "fa_host.hpp"
 
 namespace {
 
@@ -799,6 +800,19 @@ __global__ void init_half_kernel(fa::half_t* ptr, size_t n, unsigned long long s
 }
 
 }  // namespace
+
+// What the paged-cache entry points (flash_attention_paged.hip) share with this file.
+namespace fa_host {
+int fail(int code, const char* text) {
+    std::snprintf(g_last_error, sizeof(g_last_error), "%s", text);
+    return code;
+}
+void clear_error() { g_last_error[0] = 0; }
+int timed(hipStream_t stream, float* elapsed_ms, int (*launch)(void*), void* arg) {
+    return timed_launch(stream, elapsed_ms, [&]() -> int { return launch(arg); });
+}
+int device_cus() { return ::device_cus(); }
+}  // namespace fa_host
 
 extern "C" {
 

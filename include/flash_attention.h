@@ -68,7 +68,8 @@ enum {
     FA_ERR_SHAPE = 4,     /* B or H <= 0, or sizes overflow */
     FA_ERR_POINTER = 5,   /* NULL tensor pointer */
     FA_ERR_RUNTIME = 6,   /* HIP runtime / launch failure; text in fa_last_error() */
-    FA_ERR_WORKSPACE = 7  /* fa_forward_noalloc: the call needs more scratch memory than the static buffer holds */
+    FA_ERR_WORKSPACE = 7  /* fa_forward_noalloc: the call needs more scratch memory than the static buffer holds;
+                             fa_forward_shared_prefix: more than it was given */
 };
 
 /* Same work and arguments as run_tensor_flash_attention, but returns a status
@@ -266,6 +267,73 @@ const char* fa_kernel_name_general_bh(int bh, int lq, int lk, int D, int flags);
 int fa_split_ways_general(int bh, int lq, int lk, int D, int flags);
 /* The same for a call of fa_forward_block_general. */
 const char* fa_kernel_name_block_general(int lq, int lk, int D, int flags, int q_pos0, int k_pos0);
+
+/* ---------------------------------------------------------------------------
+ * Paged K/V cache: serving a batch whose requests share a long prefix
+ * (no counterpart in the reference, whose K and V are dense [B][H][L][D]
+ * tensors, flash_attention_tensor_cores/wrapper.cu:21-34)
+ * ------------------------------------------------------------------------- */
+
+/* Keys and values in pages of page_size keys (a power of two from 16 to 65536): element (page, head, row, d) of K is
+ * k[page * k_strides[0] + head * k_strides[1] + row * k_strides[2] + d], V alike.  16-bit elements, D contiguous;
+ * [n_pages][heads][page_size][D], [n_pages][page_size][heads][D] and K and V in one pool are all a choice of strides
+ * (multiples of 8 elements; offsets are 64-bit).  head_dim 64, 128 or 256. */
+typedef struct fa_paged_cache {
+    uint16_t* k;
+    uint16_t* v;
+    int64_t k_strides[3], v_strides[3];
+    int n_pages, page_size, heads, head_dim;
+} fa_paged_cache;
+
+/* The tables of one serving step, built on the GPU from the requests' lengths (all arrays are DEVICE arrays of ints).
+ *   k_len[B]       keys each request holds, in the first ceil(k_len / page_size) pages of its row of the block table
+ *   n_new[B]       keys it adds in this step, or, negative, drops from its end (-k_len: it is finished)
+ *   block_table    [B][table_width], rows table_stride entries apart; the entries of the pages added are written
+ *   free_pages     [free_cap], a stack whose first free_count[0] entries are free pages.  The pages that requests drop
+ *                  go on top in request order; then, in request order, requests take theirs from the top down.
+ * Outputs:
+ *   q_start[B + 1] where each request's new tokens begin in the packed token axis (running sum of max(n_new, 0))
+ *   k_len_out[B]   keys held after the step
+ *   slots[max_tokens]  for each token the place of its key and value, page * page_size + row; -1 from the last token on
+ *   counts[2]      free pages left, requests refused
+ * A request is refused when its pages, counted with those of every request before it, are more than there are, when
+ * its row of the table cannot name them, or when its tokens end behind max_tokens: it keeps its length, takes nothing,
+ * and its tokens' slots are -1.  Requests that need no page are never refused for want of pages.
+ * k_len, n_new and free_count must not overlap the outputs: a program alternates two sets (the free list and the table
+ * are updated in place).  B from 1 to 5120; one launch, nothing allocated, no synchronisation. */
+int fa_cache_plan(const int* k_len, const int* n_new, int* block_table, int64_t table_stride, int* free_pages,
+                  const int* free_count, int* q_start, int* k_len_out, int* slots, int* counts, int B, int table_width,
+                  int page_size, int free_cap, int max_tokens, void* stream, float* elapsed_ms);
+
+/* Stores new keys and values: row (t, h) of dK (element t * k_tok + h * k_head + d, strides multiples of 8) and of dV
+ * goes into slot slots[t] of the cache.  A slot that is negative or on a page the cache does not have is skipped.  Two
+ * tokens with one slot leave either's 16-byte pieces there. */
+int fa_cache_write(const uint16_t* dK, const uint16_t* dV, int64_t k_tok, int64_t k_head, int64_t v_tok, int64_t v_head,
+                   const fa_paged_cache* cache, const int* slots, int tokens, void* stream, float* elapsed_ms);
+
+enum { FA_DTYPE_FP16 = 0, FA_DTYPE_BF16 = 1 };
+
+/* Attention of a batch over the cache: request b's new tokens are rows q_start[b] .. q_start[b + 1] - 1 of
+ *   dQ, dO   element (t, h, d) at t * q_tok + h * q_head + d (o_tok, o_head), Hq query heads, Hq / cache->heads of which
+ *            share a K/V head, 16-bit elements of `dtype` (that of the cache)
+ * and see the prefix_len keys on the pages prefix_table names, which all requests share, and the k_len[b] keys on the
+ * pages of row b of the block table (the new tokens' own among them, the last ones): with FA_FLAG_CAUSAL new token i
+ * of n sees keys j <= k_len[b] - n + i of those.  Scores are scaled by `scale` (positive; 1/sqrt(D) as a rule).  prefix_len = 0 is plain paged attention.
+ * The prefix is read once for the batch, not once per request.
+ *   Nothing of a page behind the last key is used, whatever it holds, nor a masked key or value (infinities and NaN
+ * among them).  A table entry outside [0, n_pages) names no page: its keys take no part.  Lengths are clamped to what the table
+ * names, q_start to [0, T].  Rows that see no key are 0; rows of dO that belong to no request keep their bytes.
+ *   max_k_len: no request holds more own keys than this as far as the host knows (the launch is divided for it; a longer
+ * request is still computed in full).  prefix_len is a host number: a captured launch keeps it.
+ *   workspace: fa_shared_prefix_workspace(...) bytes, 16-byte aligned, for this call alone until it has run
+ * (FA_ERR_WORKSPACE when it is too small).  Nothing is allocated, nothing waits: the call can be captured. */
+int fa_forward_shared_prefix(const uint16_t* dQ, int64_t q_tok, int64_t q_head, uint16_t* dO, int64_t o_tok, int64_t o_head,
+                             const fa_paged_cache* cache, const int* prefix_table, int prefix_len, const int* block_table,
+                             int64_t table_stride, int table_width, const int* q_start, const int* k_len, int T, int B, int Hq,
+                             int dtype, int flags, float scale, int max_k_len, void* workspace, size_t workspace_bytes,
+                             void* stream, float* elapsed_ms);
+/* Bytes of workspace such a call takes on the current device (0 for sizes the call refuses). */
+size_t fa_shared_prefix_workspace(int T, int B, int Hq, int Hkv, int D, int prefix_len, int max_k_len);
 
 #ifdef __cplusplus
 }

@@ -5,6 +5,7 @@ cd "$(dirname "${BASH_SOURCE[0]}")/.."
 name=$1; shift
 mkdir -p build_ab
 python3 tools/check_owned_regs.py "$@"
+make -s -C flash-attention_amd/csrc flash_attention_paged.o
 /opt/rocm/bin/hipcc -O3 -std=c++17 --offload-arch=gfx950 -fno-honor-nans -fPIC -shared -Wall -Wno-unused-result "$@" \
-    -o build_ab/$name.so flash-attention_amd/csrc/flash_attention_capi.hip
+    -o build_ab/$name.so flash-attention_amd/csrc/flash_attention_capi.hip -Wl,flash-attention_amd/csrc/flash_attention_paged.o
 echo "built build_ab/$name.so"
