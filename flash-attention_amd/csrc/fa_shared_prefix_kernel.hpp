@@ -16,6 +16,7 @@
 // Rows that see no key give 0.
 #pragma once
 #include "fa_fwd_general_kernel.hpp"
+#include "fa_fwd_ring_kernel.hpp"  // wait_all_vmem
 #include "fa_paged_index.hpp"
 
 namespace fa {
@@ -38,6 +39,7 @@ struct SharedPrefixParams {
     float scale_log2e;
     int prefix_parts, prefix_range;  // key ranges of the prefix, keys per range (whole tiles)
     int own_parts, own_range;        // the same for the requests' own keys; the last range takes whatever is left
+    int prefix_tiles, own_tiles;     // row tiles per K/V head
     int prefix_blocks;               // workgroups of the prefix part: the first ones of the grid
 };
 
@@ -88,18 +90,60 @@ __device__ __forceinline__ typename Elem<E>::v8 special_part(typename Elem<E>::v
 }
 
 template <int D>
-struct SharedCfg {
-    static constexpr int kTk = 64;
-    static constexpr int kOcc = D == 256 ? 1 : 2;
+struct SharedCfg;
+template <>
+struct SharedCfg<64> {
+    static constexpr int kTk = 64, kStages = 4, kOcc = 2;  // 16 KiB a stage
 };
+template <>
+struct SharedCfg<128> {
+    static constexpr int kTk = 32, kStages = 4, kOcc = 2;  // 16 KiB
+};
+template <>
+struct SharedCfg<256> {
+    static constexpr int kTk = 32, kStages = 4, kOcc = 1;  // 32 KiB
+};
+
+// Item x of units x tiles: eight units at a time, tile by tile, so that the row tiles that read the same keys (one unit: a
+// K/V head and a range) follow each other on one XCD (workgroup ids congruent mod 8 share one and its L2).
+__device__ __forceinline__ void unit_and_tile(int x, int units, int tiles, int& unit, int& tile) {
+    const int full = units >> 3, per = 8 * tiles;
+    const int grp = min(x / per, full), r = x - grp * per, w = grp < full ? 8 : units & 7;
+    tile = r / w;
+    unit = grp * 8 + (r - tile * w);
+}
+
+// The request that owns row tile `tile`: the last b with first_row_tile(b) <= tile, 64 candidates at a time.
+__device__ __forceinline__ int request_of_tile(const SharedPrefixParams& p, int tile, int lane) {
+    int lo = 0, n = p.B;
+    do {
+        const int step = (n + 63) >> 6, i = lane * step;
+        const bool le = i < n && first_row_tile(clamp_int(p.q_start[min(lo + i, p.B)], 0, p.T), lo + i, p.g, 7) <= tile;
+        const uint64_t m = __ballot(le);
+        const int k = m ? 63 - __builtin_clzll(m) : 0;
+        lo += k * step;
+        n = min(step, n - k * step);
+    } while (n > 1);
+    return lo;
+}
+
+// global -> LDS, 16 bytes per lane: lane l's piece lands at lds + 16 l.  Hidden from the compiler (it would drain every
+// transfer in front of every LDS read); completion is awaited by hand.
+__device__ __forceinline__ void dma16(unsigned lds, const char* base, unsigned off) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds), "v"(off), "s"(base) : "memory");
+}
 
 template <typename E, int D>
 __global__ __launch_bounds__(256, SharedCfg<D>::kOcc) void fa_shared_prefix_kernel(const SharedPrefixParams p) {
     using HD = HeadDim<D>;
+    using CFG = SharedCfg<D>;
     using v8 = typename Elem<E>::v8;
-    constexpr int TK = SharedCfg<D>::kTk, KB = TK / 32, kTile = TK * HD::kRow;
-    constexpr int CHUNKS = kTile / 16 / 256, RSTEP = 256 / HD::kChunks;
-    __shared__ __attribute__((aligned(16))) char smem[4 * kTile];
+    constexpr int TK = CFG::kTk, KB = TK / 32, ST = CFG::kStages, kTile = TK * HD::kRow, kStage = 2 * kTile;
+    constexpr int PPW = kTile / 1024 / 4;            // 1 KiB pieces of a K (or V) tile that each wave moves
+    constexpr int RPP = 1024 / HD::kRow;             // rows per piece
+    constexpr int RPW = RPP * PPW;                   // rows per wave and tile: 16 (D = 64) or 8, on one page
+    constexpr int CPT = TK / 16;                     // 16-key groups per tile
+    __shared__ __attribute__((aligned(1024))) char ring[ST * kStage];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const LaneGeomD<D> geo = make_lane_geom_d<D>(lane);
@@ -107,36 +151,24 @@ __global__ __launch_bounds__(256, SharedCfg<D>::kOcc) void fa_shared_prefix_kern
 
     // ---- which rows against which keys
     const bool own = (int)blockIdx.x >= p.prefix_blocks;
-    int tile, head, part;
-    int row0, rows;              // stacked rows of this tile's request (or of the whole batch), and how many
-    int tok0 = 0, n_tok, keys, key0, key1;
+    int tile, head, part, row0, rows, tok0 = 0, n_tok, keys, key0, key1, table_n;
     const int* table;
-    int table_n;
     {
         const int parts = own ? p.own_parts : p.prefix_parts;
-        int x = (int)blockIdx.x - (own ? p.prefix_blocks : 0);
-        part = x % parts;
-        x /= parts;
-        head = x % p.Hkv;
-        tile = x / p.Hkv;
+        int unit;
+        unit_and_tile((int)blockIdx.x - (own ? p.prefix_blocks : 0), p.Hkv * parts, own ? p.own_tiles : p.prefix_tiles, unit, tile);
+        head = unit / parts;
+        part = unit - head * parts;
         if (own) {
-            int lo = 0, hi = p.B;
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (first_row_tile(clamp_int(p.q_start[mid], 0, p.T), mid, p.g, 7) <= tile)
-                    lo = mid;
-                else
-                    hi = mid;
-            }
-            tok0 = clamp_int(p.q_start[lo], 0, p.T);
-            n_tok = clamp_int(p.q_start[lo + 1], tok0, p.T) - tok0;
-            tile -= first_row_tile(tok0, lo, p.g, 7);
-            table = p.block_table + lo * p.table_stride;
+            const int b = __builtin_amdgcn_readfirstlane(request_of_tile(p, tile, lane));
+            tok0 = clamp_int(p.q_start[b], 0, p.T);
+            n_tok = clamp_int(p.q_start[b + 1], tok0, p.T) - tok0;
+            tile -= first_row_tile(tok0, b, p.g, 7);
+            table = p.block_table + b * p.table_stride;
             table_n = p.table_width;
-            const int64_t room = (int64_t)p.table_width << p.log2_page;
-            keys = clamp_int(p.k_len[lo], 0, (int)room);
-            key0 = (int)min((int64_t)part * p.own_range, (int64_t)keys);
-            key1 = part == p.own_parts - 1 ? keys : (int)min((int64_t)key0 + p.own_range, (int64_t)keys);
+            keys = clamp_int(p.k_len[b], 0, p.table_width << p.log2_page);
+            key0 = min(part * p.own_range, keys);  // (parts * range is below 2^31: the launcher's check)
+            key1 = part == p.own_parts - 1 ? keys : min(key0 + p.own_range, keys);
         } else {
             n_tok = clamp_int(p.q_start[p.B], 0, p.T);
             table = p.prefix_table;
@@ -150,13 +182,11 @@ __global__ __launch_bounds__(256, SharedCfg<D>::kOcc) void fa_shared_prefix_kern
         if (tile < 0 || row0 >= rows) return;
     }
     const bool causal = own && p.causal != 0;
-    const int part_all = own ? p.prefix_parts + part : part;
     const int R = min(row0 + wave * 32 + geo.r, rows - 1);  // this lane's row; past the end the last one, not stored
     const bool valid = row0 + wave * 32 + geo.r < rows;
     const bool wave_valid = row0 + wave * 32 < rows;
     const int ti = R / p.g, tok = tok0 + ti, hq = head * p.g + (R - ti * p.g);
     const int Hq = p.Hkv * p.g;
-    const int64_t slot = (int64_t)part_all * p.T * Hq + (int64_t)tok * Hq + hq;
     // the last key this row sees; a workgroup need not walk past its last row's
     const int limit = causal ? min(keys - 1, keys - n_tok + ti) : keys - 1;
     if (causal) {
@@ -164,6 +194,52 @@ __global__ __launch_bounds__(256, SharedCfg<D>::kOcc) void fa_shared_prefix_kern
         key1 = min(key1, keys - n_tok + last_ti + 1);
     }
     const int n_tiles = key1 > key0 ? (key1 - key0 + TK - 1) / TK : 0;
+
+    // ---- transfers: this wave moves rows RPW * wave .. of each tile.  They lie on one page, whose number is uniform: lane L
+    //      holds the entry of the 16-key group group0 + L of the range, 64 groups at a time (the next 64 are loaded one
+    //      refill ahead).  Lane l fills slot l % kChunks of row l / kChunks of a piece with the chunk the swizzle maps there.
+    const unsigned ring_lds = __builtin_amdgcn_readfirstlane((unsigned)(size_t)(__attribute__((address_space(3))) char*)ring);
+    const int d_rip = lane / HD::kChunks, d_slot = lane % HD::kChunks;
+    unsigned k_off[PPW], v_off[PPW];
+#pragma unroll
+    for (int j = 0; j < PPW; ++j) {
+        const int row = RPW * wave + RPP * j + d_rip;
+        k_off[j] = (unsigned)((RPP * j + d_rip) * (int)p.ks.row * 2) + (unsigned)((d_slot ^ (row & HD::kKMask)) << 4);
+        v_off[j] = (unsigned)((RPP * j + d_rip) * (int)p.vs.row * 2) + (unsigned)((d_slot ^ ((row & HD::kVMask) << 2)) << 4);
+    }
+    const char* k_head = reinterpret_cast<const char*>(p.kc + head * p.ks.head);
+    const char* v_head = reinterpret_cast<const char*>(p.vc + head * p.vs.head);
+    auto load_pages = [&](int group) -> int {  // -1: no page
+        const int j = (key0 + 16 * (group + lane)) >> p.log2_page;
+        const int page = j < table_n ? table[j] : -1;
+        return page_ok(page, p.n_pages) ? page : -1;
+    };
+    int pages = 0, pages_next = 0;
+    unsigned on_page = 0;  // CPT bits per tile sent for and not yet computed: the groups that lie on a page
+    auto send = [&](int t) {
+        const int g0 = t * CPT;
+        if ((g0 & 63) == 0) {
+            pages = t == 0 ? load_pages(0) : pages_next;
+            pages_next = load_pages(g0 + 64);
+        }
+        on_page |= ((unsigned)(__ballot(pages >= 0) >> (g0 & 63)) & ((1u << CPT) - 1)) << (CPT * (ST - 1));
+        // (a group on no page is fetched from page 0: its scores are masked)
+        const int page = max(__builtin_amdgcn_readlane(pages, (g0 + wave * RPW / 16) & 63), 0);
+        const int row = (key0 + t * TK + wave * RPW) & P1;
+        const char* kb = k_head + 2 * ((int64_t)page * p.ks.page + (int64_t)row * p.ks.row);
+        const char* vb = v_head + 2 * ((int64_t)page * p.vs.page + (int64_t)row * p.vs.row);
+        const unsigned l = ring_lds + (unsigned)(t % ST) * kStage + (unsigned)(PPW * wave) * 1024u;
+#pragma unroll
+        for (int j = 0; j < PPW; ++j) dma16(l + 1024u * j, kb, k_off[j]);
+#pragma unroll
+        for (int j = 0; j < PPW; ++j) dma16(l + kTile + 1024u * j, vb, v_off[j]);
+    };
+
+#pragma unroll
+    for (int t = 0; t < ST - 1; ++t) {
+        if (t < n_tiles) send(t);
+        on_page >>= CPT;
+    }
 
     v8 qf[HD::kSteps];
     {
@@ -179,31 +255,6 @@ __global__ __launch_bounds__(256, SharedCfg<D>::kOcc) void fa_shared_prefix_kern
 #pragma unroll
         for (int e = 0; e < 16; ++e) oacc[db][e] = 0.0f;
 
-    const int st_row = tid / HD::kChunks, st_ch = tid % HD::kChunks;
-    u32x4 st_k[CHUNKS], st_v[CHUNKS];
-    // the page of a key, -1 where there is none; a row on no page is fetched from page 0: its score is masked
-    auto page_of = [&](int key) -> int {
-        const int j = key >> p.log2_page;
-        const int page = j < table_n ? table[j] : -1;
-        return page_ok(page, p.n_pages) ? page : -1;
-    };
-    auto stage_load = [&](int t) {
-#pragma unroll
-        for (int i = 0; i < CHUNKS; ++i) {
-            const int key = key0 + t * TK + st_row + i * RSTEP, page = max(page_of(key), 0);
-            st_k[i] = *reinterpret_cast<const u32x4*>(p.kc + cache_offset(p.ks, page, head, key & P1) + st_ch * 8);
-            st_v[i] = *reinterpret_cast<const u32x4*>(p.vc + cache_offset(p.vs, page, head, key & P1) + st_ch * 8);
-        }
-    };
-    auto stage_write = [&](int buf) {
-        char* kw = smem + buf * 2 * kTile;
-#pragma unroll
-        for (int i = 0; i < CHUNKS; ++i) {
-            const int row = st_row + i * RSTEP;
-            *reinterpret_cast<u32x4*>(kw + row * HD::kRow + ((st_ch ^ (row & HD::kKMask)) << 4)) = st_k[i];
-            *reinterpret_cast<u32x4*>(kw + kTile + row * HD::kRow + ((st_ch ^ ((row & HD::kVMask) << 2)) << 4)) = st_v[i];
-        }
-    };
     auto v_frag = [&](const char* vb, int kk, int db) -> v8 {
         const char* a0 = vb + geo.v_rd[db] + kk * 16 * HD::kRow;
         const short4_t t0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t*)(a0));
@@ -211,17 +262,16 @@ __global__ __launch_bounds__(256, SharedCfg<D>::kOcc) void fa_shared_prefix_kern
         return __builtin_bit_cast(v8, __builtin_shufflevector(t0, t1, 0, 1, 2, 3, 4, 5, 6, 7));
     };
 
-    if (n_tiles > 0) {
-        stage_load(0);
-        stage_write(0);
-    }
+    wait_all_vmem();
     __syncthreads();
     for (int t = 0; t < n_tiles; ++t) {
-        if (t + 1 < n_tiles) stage_load(t + 1);
+        const unsigned groups = on_page & ((1u << CPT) - 1);
+        if (t + ST - 1 < n_tiles) send(t + ST - 1);  // into the stage of tile t - 1, which every wave has left
+        on_page >>= CPT;
+        const int first = key0 + t * TK;
         if (wave_valid) {
-            const char* kb = smem + (t & 1) * 2 * kTile;
+            const char* kb = ring + (t % ST) * kStage;
             const char* vb = kb + kTile;
-            const int first = key0 + t * TK;
             f32x16 s[KB];
 #pragma unroll
             for (int b = 0; b < KB; ++b) {
@@ -231,12 +281,8 @@ __global__ __launch_bounds__(256, SharedCfg<D>::kOcc) void fa_shared_prefix_kern
                 for (int ks = 0; ks < HD::kSteps; ++ks)
                     s[b] = Elem<E>::mfma(*reinterpret_cast<const v8*>(kb + geo.k_rd[ks] + b * 32 * HD::kRow), qf[ks], s[b]);
             }
-            // which 16-key groups of the tile lie on a page
-            unsigned groups = 0;
-#pragma unroll
-            for (int c = 0; c < TK / 16; ++c) groups |= page_of(first + 16 * c) >= 0 ? 1u << c : 0u;
             const int lim = min(limit, key1 - 1) - first;
-            const bool masked = __any(lim < TK - 1) || groups != (1u << (TK / 16)) - 1;
+            const bool masked = __any(lim < TK - 1) || groups != (1u << CPT) - 1;
             if (masked) {
 #pragma unroll
                 for (int b = 0; b < KB; ++b)
@@ -250,7 +296,7 @@ __global__ __launch_bounds__(256, SharedCfg<D>::kOcc) void fa_shared_prefix_kern
 #pragma unroll
             for (int b = 0; b < KB; ++b)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) mx = max_nan(mx, s[b][e]);
+                for (int e = b == 0 ? 1 : 0; e < 16; ++e) mx = max_nan(mx, s[b][e]);
             {
                 float a, b;
                 half_wave_pair(mx, a, b);
@@ -295,6 +341,7 @@ __global__ __launch_bounds__(256, SharedCfg<D>::kOcc) void fa_shared_prefix_kern
                             const int k = 16 * kk + 8 * (i >> 2) + (i & 3);
                             sees[kk][i] = (E)(k + 4 * geo.hh <= lim && ((groups >> (k >> 4)) & 1) ? 1.0f : 0.0f);
                         }
+#pragma unroll 1
                     for (int kind = 1; kind <= 3; ++kind) {
                         const unsigned bits = kind == 1 ? 0x7fc00000u : kind == 2 ? 0x7f800000u : 0xff800000u;
 #pragma unroll
@@ -313,11 +360,16 @@ __global__ __launch_bounds__(256, SharedCfg<D>::kOcc) void fa_shared_prefix_kern
                 }
             }
         }
-        if (t + 1 < n_tiles) stage_write((t + 1) & 1);
+        // this wave's share of tile t + 1 has landed (transfers complete in order); the next ST - 2 stay in flight
+        if (t + ST - 1 < n_tiles)
+            asm volatile("s_waitcnt vmcnt(%0)" : : "n"((ST - 2) * 2 * PPW) : "memory");
+        else
+            wait_all_vmem();
         __syncthreads();
     }
 
     if (!valid) return;
+    const int64_t slot = (int64_t)(own ? p.prefix_parts + part : part) * p.T * Hq + (int64_t)tok * Hq + hq;
     float l0, l1;
     half_wave_pair(l_run, l0, l1);
     if (geo.hh == 0) {

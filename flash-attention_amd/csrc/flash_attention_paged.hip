@@ -61,6 +61,8 @@ int check_cache(const fa_paged_cache* c) {
     if (!aligned16({c->k, c->v}) ||
         !whole_pieces({c->k_strides[0], c->k_strides[1], c->k_strides[2], c->v_strides[0], c->v_strides[1], c->v_strides[2]}))
         return fail(FA_ERR_SHAPE, "paged cache: k and v must be 16-byte aligned, strides multiples of 8 elements");
+    if (c->k_strides[2] > (1 << 25) || c->v_strides[2] > (1 << 25))  // (the lanes' offsets within 16 rows are 32-bit)
+        return fail(FA_ERR_SHAPE, "paged cache: row strides must be at most 2^25 elements");
     return FA_OK;
 }
 fa::CacheStrides strides_of(const int64_t (&s)[3]) { return {s[0], s[1], s[2]}; }
@@ -229,6 +231,7 @@ int fa_forward_shared_prefix(const uint16_t* dQ, int64_t q_tok, int64_t q_head, 
     p.prefix_len = prefix_len, p.table_width = table_width, p.causal = flags & FA_FLAG_CAUSAL;
     p.scale_log2e = scale * 1.44269504088896340736f;
     p.prefix_parts = d.prefix_parts, p.prefix_range = d.prefix_range, p.own_parts = d.own_parts, p.own_range = d.own_range;
+    p.prefix_tiles = d.prefix_tiles, p.own_tiles = d.own_tiles;
     const int64_t prefix_blocks = (int64_t)d.prefix_tiles * Hkv * d.prefix_parts;
     if (prefix_blocks > 0x7fffffffLL) return fail(FA_ERR_SHAPE, "fa_forward_shared_prefix: grid size out of range");
     p.prefix_blocks = (int)prefix_blocks;
