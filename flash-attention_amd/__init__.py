@@ -552,7 +552,7 @@ def attention_shared_prefix(q, cache: PagedCache, q_start, k_len, block_table, p
     tokens (any token and head strides; Hq a multiple of the cache's heads), request b's being rows ``q_start[b]`` to
     ``q_start[b + 1]``; they see the ``prefix_len`` keys on the pages of ``prefix_table`` and the request's own ``k_len[b]``
     keys on the pages of ``block_table[b]``, the new tokens' own among them (already written), with ``causal`` only up to their
-    own.  ``max_k_len``: a bound on ``k_len`` that the launch is divided for (default: what the table names).  Rows of
+    own.  ``max_k_len``: a bound on ``k_len`` that the workspace is made for (default: what the table names).  Rows of
     ``out`` that belong to no request are left as they are (0 in a new one).  Returns ``out`` (and the kernel-only
     milliseconds when ``timed``)."""
     import torch

@@ -1,5 +1,5 @@
-// Index arithmetic of the paged K/V cache: which page a key lies in, where a cache row is in memory, which request a
-// tile of query rows belongs to.  Plain functions of whole numbers for host and device: the kernels take every bound
+// Index arithmetic of the paged K/V cache: which page a key lies in, where a cache row is in memory, how many workgroups a
+// launch can need.  Plain functions of whole numbers for host and device: the kernels take every bound
 // from here, and the CPU tests run the same code (tests/cpp/paged_index_check.cpp).
 //
 // A cache is [n_pages][Hkv][page_size][D] with any strides of the first three axes (so token-major pages are a
@@ -37,15 +37,27 @@ FA_HD int slot_of(int page, int row, int log2_page) {
     return page < 0 || s > 0x7fffffffLL ? -1 : (int)s;
 }
 
-// Rows of request b (its new tokens times the query heads that share a K/V head) in tiles of 2^log2_rows: tile x of the
-// batch is tile x - first_row_tile(b) of the request with the largest first_row_tile(b) <= x.  The sums
-// floor(rows before b / tile) + b leave every request room for its own tiles, whatever the lengths; tiles past a
-// request's last row are empty.
-FA_HD int first_row_tile(int q_start_b, int b, int group, int log2_rows) {
-    return (int)(((int64_t)q_start_b * group) >> log2_rows) + b;
+// How a launch of shared-prefix attention is divided.  Row tiles of 128 rows walk `tiles` key tiles each, in `parts_for`
+// ranges of about `steps_for` key tiles: all key tiles of the launch (`work`, per K/V head) over the workgroups that the
+// chip holds (`slots`).  With x = tiles / steps a row tile has max(1, floor(x + 1/2)) ranges at most, i.e. fewer than x
+// beyond the first, and all x together are at most `slots`: blocks_bound holds for any lengths (with half as much again for
+// the rounding of the sum).
+constexpr int kRowTile = 128;
+FA_HD int row_tiles(int64_t rows) { return (int)((rows + kRowTile - 1) / kRowTile); }
+FA_HD int parts_for(int tiles, int steps, int most) {
+    int n = (int)(((int64_t)tiles + (steps >> 1)) / steps);
+    if (n > most) n = most;
+    return n < 1 ? 1 : n;
 }
-FA_HD int row_tiles_bound(int tokens, int requests, int group, int log2_rows) {
-    return (int)(((int64_t)tokens * group) >> log2_rows) + requests;
+FA_HD int steps_for(float work, int heads, int slots, int least) {
+    const float per = work * (float)heads / (float)slots;
+    const int n = (int)(per < 1e9f ? per : 1e9f) + 1;
+    return n < least ? least : n;
+}
+// Row tiles of a batch of `requests` with `rows` rows in all, and its workgroups.
+FA_HD int64_t request_tiles_bound(int64_t rows, int requests) { return rows / kRowTile + requests; }
+FA_HD int64_t blocks_bound(int64_t prefix_row_tiles, int64_t request_row_tiles, int heads, int slots) {
+    return heads * (prefix_row_tiles + request_row_tiles) + 3 * (int64_t)slots / 2 + 1;
 }
 
 // One request's step, from its lengths alone.  keys held (clamped to what a table row names), keys after the step,

@@ -33,14 +33,13 @@ struct SharedPrefixParams {
     int64_t table_stride;
     const int* q_start;
     const int* k_len;
-    float* part_o;   // [parts][T * Hq][D], un-normalised
-    float* part_ml;  // [parts][T * Hq][2]: largest score (log2 units) and sum of exp2(score - largest)
+    float* part_o;    // [parts][T * Hq][D], un-normalised
+    float* part_ml;   // [parts][T * Hq][2]: largest score (log2 units) and sum of exp2(score - largest)
+    int* row_parts;   // [T * Hq]: parts of the row's sum; 0: its output is written already
     int T, B, Hkv, g, log2_page, n_pages, prefix_len, table_width, causal;
     float scale_log2e;
-    int prefix_parts, prefix_range;  // key ranges of the prefix, keys per range (whole tiles)
-    int own_parts, own_range;        // the same for the requests' own keys; the last range takes whatever is left
-    int prefix_tiles, own_tiles;     // row tiles per K/V head
-    int prefix_blocks;               // workgroups of the prefix part: the first ones of the grid
+    int slots;                      // workgroups that the chip holds at a time
+    int max_prefix_parts, max_own_parts;
 };
 
 template <typename E>
@@ -104,6 +103,104 @@ struct SharedCfg<256> {
     static constexpr int kTk = 32, kStages = 4, kOcc = 1;  // 32 KiB
 };
 
+// The division of a launch into workgroups, from the requests' lengths; every workgroup computes it for itself.
+//   A request with fewer than 128 rows (new tokens x g) is short: its rows are stacked up with those of the other short
+// requests against the prefix (items of kind P: one K/V head, 128 stacked rows, a range of the prefix) and alone against
+// its own keys (O: one head, the request's rows, a range of its keys).  A longer request fills row tiles of its own, which walk
+// prefix and own keys in one go (J: one head, 128 of its rows, a range of both): nothing is gained by stacking.
+//   Ranges are `steps` key tiles long, up to half a range more or less: all tiles of the launch over the workgroups that
+// the chip holds.
+struct SharedPlan {
+    int stacked;        // rows of the short requests, per K/V head
+    int prefix_tiles;   // key tiles of the prefix
+    int prefix_parts;   // ranges of the prefix that P items walk
+    int p_items;
+    int steps;
+};
+
+// Inclusive sum over the 256 threads of a workgroup; `total` for everybody.  `tmp`: 4 ints of LDS.
+__device__ __forceinline__ int workgroup_sum(int v, int* tmp, int& total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int u = __shfl_up(v, d);
+        if (lane >= d) v += u;
+    }
+    __syncthreads();
+    if (lane == 63) tmp[wave] = v;
+    __syncthreads();
+    const int a = tmp[0], b = tmp[1], c = tmp[2];
+    total = a + b + c + tmp[3];
+    return v + (wave > 0 ? a : 0) + (wave > 1 ? b : 0) + (wave > 2 ? c : 0);
+}
+
+struct SharedRequest {
+    int tok0, n, keys;
+};
+__device__ __forceinline__ SharedRequest shared_request(const SharedPrefixParams& p, int b) {
+    SharedRequest r;
+    r.tok0 = clamp_int(p.q_start[b], 0, p.T);
+    r.n = clamp_int(p.q_start[b + 1], r.tok0, p.T) - r.tok0;
+    r.keys = clamp_int(p.k_len[b], 0, p.table_width << p.log2_page);
+    return r;
+}
+
+// Items of a request; 0 where it has no rows.
+template <int TK>
+__device__ __forceinline__ int request_items(const SharedPrefixParams& p, const SharedPlan& s, const SharedRequest& r, int& tiles, int& parts) {
+    const int rows = r.n * p.g, own = (r.keys + TK - 1) / TK;
+    tiles = (rows + 127) >> 7;
+    parts = rows >= 128 ? parts_for(s.prefix_tiles + own, s.steps, p.max_prefix_parts + p.max_own_parts) : parts_for(own, s.steps, p.max_own_parts);
+    return tiles * parts * p.Hkv;
+}
+
+// LDS: stacked_start[B] (stacked tokens before request b), item_start[B] (items before it, P items among them).
+template <int TK>
+__device__ __forceinline__ int shared_plan(const SharedPrefixParams& p, SharedPlan& s, int* stacked_start, int* item_start, int* tmp) {
+    s.prefix_tiles = (p.prefix_len + TK - 1) / TK;
+    int tokens = 0;
+    float work = 0.0f;  // key tiles of all row tiles, per K/V head
+    for (int b0 = 0; b0 < p.B; b0 += 256) {
+        const int b = b0 + (int)threadIdx.x;
+        int n = 0;
+        if (b < p.B) {
+            const SharedRequest r = shared_request(p, b);
+            const int rows = r.n * p.g, own = (r.keys + TK - 1) / TK;
+            if (rows < 128) n = r.n;
+            work += (float)((rows + 127) >> 7) * (float)(own + (rows < 128 ? 0 : s.prefix_tiles));
+        }
+        int total;
+        const int sum = workgroup_sum(n, tmp, total);
+        if (b < p.B) stacked_start[b] = tokens + sum - n;
+        tokens += total;
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) work += __shfl_xor(work, d);
+    float* ftmp = reinterpret_cast<float*>(tmp);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) ftmp[threadIdx.x >> 6] = work;
+    __syncthreads();
+    work = ftmp[0] + ftmp[1] + ftmp[2] + ftmp[3];
+    s.stacked = tokens * p.g;
+    const int p_tiles = (s.stacked + 127) >> 7;
+    work += (float)p_tiles * (float)s.prefix_tiles;
+    s.steps = steps_for(work, p.Hkv, p.slots, 128 / TK);
+    s.prefix_parts = s.prefix_tiles > 0 && p_tiles > 0 ? parts_for(s.prefix_tiles, s.steps, p.max_prefix_parts) : 0;
+    s.p_items = p_tiles * s.prefix_parts * p.Hkv;
+    int items = s.p_items;
+    for (int b0 = 0; b0 < p.B; b0 += 256) {
+        const int b = b0 + (int)threadIdx.x;
+        int n = 0, tiles, parts;
+        if (b < p.B) n = request_items<TK>(p, s, shared_request(p, b), tiles, parts);
+        int total;
+        const int sum = workgroup_sum(n, tmp, total);
+        if (b < p.B) item_start[b] = items + sum - n;
+        items += total;
+    }
+    __syncthreads();
+    return items;
+}
+
 // Item x of units x tiles: eight units at a time, tile by tile, so that the row tiles that read the same keys (one unit: a
 // K/V head and a range) follow each other on one XCD (workgroup ids congruent mod 8 share one and its L2).
 __device__ __forceinline__ void unit_and_tile(int x, int units, int tiles, int& unit, int& tile) {
@@ -113,18 +210,18 @@ __device__ __forceinline__ void unit_and_tile(int x, int units, int tiles, int& 
     unit = grp * 8 + (r - tile * w);
 }
 
-// The request that owns row tile `tile`: the last b with first_row_tile(b) <= tile, 64 candidates at a time.
-__device__ __forceinline__ int request_of_tile(const SharedPrefixParams& p, int tile, int lane) {
-    int lo = 0, n = p.B;
-    do {
+// The last b with start[b] <= x, 64 candidates at a time (start in LDS, ascending, start[0] <= x; x uniform).
+__device__ __forceinline__ int last_at_most(const int* start, int count, int x) {
+    const int lane = threadIdx.x & 63;
+    int lo = 0, n = count;
+    while (n > 1) {
         const int step = (n + 63) >> 6, i = lane * step;
-        const bool le = i < n && first_row_tile(clamp_int(p.q_start[min(lo + i, p.B)], 0, p.T), lo + i, p.g, 7) <= tile;
-        const uint64_t m = __ballot(le);
-        const int k = m ? 63 - __builtin_clzll(m) : 0;
+        const uint64_t m = __ballot(i < n && start[min(lo + i, count - 1)] <= x);
+        const int k = 63 - __builtin_clzll(m);
         lo += k * step;
         n = min(step, n - k * step);
-    } while (n > 1);
-    return lo;
+    }
+    return __builtin_amdgcn_readfirstlane(lo);
 }
 
 // global -> LDS, 16 bytes per lane: lane l's piece lands at lds + 16 l.  Hidden from the compiler (it would drain every
@@ -147,53 +244,56 @@ __global__ __launch_bounds__(256, SharedCfg<D>::kOcc) void fa_shared_prefix_kern
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const LaneGeomD<D> geo = make_lane_geom_d<D>(lane);
-    const int P1 = (1 << p.log2_page) - 1;
+    const int P1 = (1 << p.log2_page) - 1;  // (row in a page)
 
-    // ---- which rows against which keys
-    const bool own = (int)blockIdx.x >= p.prefix_blocks;
-    int tile, head, part, row0, rows, tok0 = 0, n_tok, keys, key0, key1, table_n;
-    const int* table;
+    // ---- which rows against which keys: rows row0 .. of a request's `rows` (or of the stacked ones) against key tiles
+    //      u0 .. of the sequence of the prefix' tiles and the request's own
+    SharedPlan plan;
+    int head, part, parts, row0, rows, u0, n_tiles, own_keys = 0, n_tok = 0, tok;
+    bool stacked;
+    const int* own_table = nullptr;
+    const int R_off = wave * 32 + geo.r;
     {
-        const int parts = own ? p.own_parts : p.prefix_parts;
-        int unit;
-        unit_and_tile((int)blockIdx.x - (own ? p.prefix_blocks : 0), p.Hkv * parts, own ? p.own_tiles : p.prefix_tiles, unit, tile);
-        head = unit / parts;
-        part = unit - head * parts;
-        if (own) {
-            const int b = __builtin_amdgcn_readfirstlane(request_of_tile(p, tile, lane));
-            tok0 = clamp_int(p.q_start[b], 0, p.T);
-            n_tok = clamp_int(p.q_start[b + 1], tok0, p.T) - tok0;
-            tile -= first_row_tile(tok0, b, p.g, 7);
-            table = p.block_table + b * p.table_stride;
-            table_n = p.table_width;
-            keys = clamp_int(p.k_len[b], 0, p.table_width << p.log2_page);
-            key0 = min(part * p.own_range, keys);  // (parts * range is below 2^31: the launcher's check)
-            key1 = part == p.own_parts - 1 ? keys : min(key0 + p.own_range, keys);
+        int* stacked_start = reinterpret_cast<int*>(ring);  // (free until the first transfer)
+        int* item_start = stacked_start + p.B;
+        __shared__ int tmp[4];
+        const int x = (int)blockIdx.x;
+        if (x >= shared_plan<TK>(p, plan, stacked_start, item_start, tmp)) return;
+        int unit, tile, u1;
+        stacked = x < plan.p_items;
+        if (stacked) {
+            parts = plan.prefix_parts;
+            unit_and_tile(x, p.Hkv * parts, (plan.stacked + 127) >> 7, unit, tile);
+            head = unit / parts, part = unit - head * parts;
+            row0 = tile * 128, rows = plan.stacked;
+            u0 = (int)((int64_t)plan.prefix_tiles * part / parts);
+            u1 = (int)((int64_t)plan.prefix_tiles * (part + 1) / parts);
+            const int t = min(row0 + R_off, rows - 1) / p.g;  // stacked token
+            const int b = owner_of(stacked_start, p.B, t);
+            tok = clamp_int(p.q_start[b], 0, p.T) + t - stacked_start[b];
         } else {
-            n_tok = clamp_int(p.q_start[p.B], 0, p.T);
-            table = p.prefix_table;
-            table_n = pages_for(p.prefix_len, p.log2_page);
-            keys = p.prefix_len;
-            key0 = part * p.prefix_range;
-            key1 = min(key0 + p.prefix_range, keys);
+            const int b = last_at_most(item_start, p.B, x);
+            const SharedRequest r = shared_request(p, b);
+            int tiles;
+            request_items<TK>(p, plan, r, tiles, parts);
+            unit_and_tile(x - item_start[b], p.Hkv * parts, tiles, unit, tile);
+            head = unit / parts, part = unit - head * parts;
+            row0 = tile * 128, rows = r.n * p.g, n_tok = r.n;
+            own_keys = r.keys;
+            own_table = p.block_table + b * p.table_stride;
+            tok = r.tok0 + min(row0 + R_off, rows - 1) / p.g;
+            // no row of the tile sees further than its last one
+            const int last_ti = (min(row0 + 128, rows) - 1) / p.g, see = p.causal ? min(r.keys, r.keys - r.n + last_ti + 1) : r.keys;
+            const int first = rows >= 128 ? 0 : plan.prefix_tiles, n = plan.prefix_tiles + (max(see, 0) + TK - 1) / TK - first;
+            u0 = first + (int)((int64_t)n * part / parts);
+            u1 = first + (int)((int64_t)n * (part + 1) / parts);
         }
-        row0 = tile * 128;
-        rows = n_tok * p.g;
-        if (tile < 0 || row0 >= rows) return;
+        n_tiles = u1 - u0;
+        __syncthreads();  // (the tables above have been read)
     }
-    const bool causal = own && p.causal != 0;
-    const int R = min(row0 + wave * 32 + geo.r, rows - 1);  // this lane's row; past the end the last one, not stored
-    const bool valid = row0 + wave * 32 + geo.r < rows;
-    const bool wave_valid = row0 + wave * 32 < rows;
-    const int ti = R / p.g, tok = tok0 + ti, hq = head * p.g + (R - ti * p.g);
-    const int Hq = p.Hkv * p.g;
-    // the last key this row sees; a workgroup need not walk past its last row's
-    const int limit = causal ? min(keys - 1, keys - n_tok + ti) : keys - 1;
-    if (causal) {
-        const int last_ti = (min(row0 + 128, rows) - 1) / p.g;
-        key1 = min(key1, keys - n_tok + last_ti + 1);
-    }
-    const int n_tiles = key1 > key0 ? (key1 - key0 + TK - 1) / TK : 0;
+    const bool valid = row0 + R_off < rows, wave_valid = row0 + wave * 32 < rows;
+    const int R = min(row0 + R_off, rows - 1), ti = R / p.g, hq = head * p.g + (R - ti * p.g), Hq = p.Hkv * p.g;
+    const int own_limit = p.causal ? min(own_keys - 1, own_keys - n_tok + ti) : own_keys - 1;  // the last own key this row sees
 
     // ---- transfers: this wave moves rows RPW * wave .. of each tile.  They lie on one page, whose number is uniform: lane L
     //      holds the entry of the 16-key group group0 + L of the range, 64 groups at a time (the next 64 are loaded one
@@ -209,9 +309,12 @@ __global__ __launch_bounds__(256, SharedCfg<D>::kOcc) void fa_shared_prefix_kern
     }
     const char* k_head = reinterpret_cast<const char*>(p.kc + head * p.ks.head);
     const char* v_head = reinterpret_cast<const char*>(p.vc + head * p.vs.head);
+    const int own_entries = p.table_width, prefix_entries = pages_for(p.prefix_len, p.log2_page);
     auto load_pages = [&](int group) -> int {  // -1: no page
-        const int j = (key0 + 16 * (group + lane)) >> p.log2_page;
-        const int page = j < table_n ? table[j] : -1;
+        const int i = group + lane, u = u0 + i / CPT, key = (u < plan.prefix_tiles ? u : u - plan.prefix_tiles) * TK + 16 * (i % CPT);
+        const int* table = u < plan.prefix_tiles ? p.prefix_table : own_table;
+        const int j = key >> p.log2_page;
+        const int page = i < n_tiles * CPT && j < (u < plan.prefix_tiles ? prefix_entries : own_entries) ? table[j] : -1;
         return page_ok(page, p.n_pages) ? page : -1;
     };
     int pages = 0, pages_next = 0;
@@ -220,12 +323,12 @@ __global__ __launch_bounds__(256, SharedCfg<D>::kOcc) void fa_shared_prefix_kern
         const int g0 = t * CPT;
         if ((g0 & 63) == 0) {
             pages = t == 0 ? load_pages(0) : pages_next;
-            pages_next = load_pages(g0 + 64);
+            pages_next = g0 + 64 < n_tiles * CPT ? load_pages(g0 + 64) : -1;
         }
         on_page |= ((unsigned)(__ballot(pages >= 0) >> (g0 & 63)) & ((1u << CPT) - 1)) << (CPT * (ST - 1));
         // (a group on no page is fetched from page 0: its scores are masked)
         const int page = max(__builtin_amdgcn_readlane(pages, (g0 + wave * RPW / 16) & 63), 0);
-        const int row = (key0 + t * TK + wave * RPW) & P1;
+        const int u = u0 + t, row = ((u < plan.prefix_tiles ? u : u - plan.prefix_tiles) * TK + wave * RPW) & P1;
         const char* kb = k_head + 2 * ((int64_t)page * p.ks.page + (int64_t)row * p.ks.row);
         const char* vb = v_head + 2 * ((int64_t)page * p.vs.page + (int64_t)row * p.vs.row);
         const unsigned l = ring_lds + (unsigned)(t % ST) * kStage + (unsigned)(PPW * wave) * 1024u;
@@ -268,8 +371,10 @@ __global__ __launch_bounds__(256, SharedCfg<D>::kOcc) void fa_shared_prefix_kern
         const unsigned groups = on_page & ((1u << CPT) - 1);
         if (t + ST - 1 < n_tiles) send(t + ST - 1);  // into the stage of tile t - 1, which every wave has left
         on_page >>= CPT;
-        const int first = key0 + t * TK;
-        if (wave_valid) {
+        const int u = u0 + t;
+        // the last key of this tile that the row sees; a wave whose rows see none of it passes it by
+        const int lim = u < plan.prefix_tiles ? p.prefix_len - 1 - u * TK : own_limit - (u - plan.prefix_tiles) * TK;
+        if (wave_valid && __any(lim >= 0)) {
             const char* kb = ring + (t % ST) * kStage;
             const char* vb = kb + kTile;
             f32x16 s[KB];
@@ -281,7 +386,6 @@ __global__ __launch_bounds__(256, SharedCfg<D>::kOcc) void fa_shared_prefix_kern
                 for (int ks = 0; ks < HD::kSteps; ++ks)
                     s[b] = Elem<E>::mfma(*reinterpret_cast<const v8*>(kb + geo.k_rd[ks] + b * 32 * HD::kRow), qf[ks], s[b]);
             }
-            const int lim = min(limit, key1 - 1) - first;
             const bool masked = __any(lim < TK - 1) || groups != (1u << CPT) - 1;
             if (masked) {
 #pragma unroll
@@ -369,13 +473,30 @@ __global__ __launch_bounds__(256, SharedCfg<D>::kOcc) void fa_shared_prefix_kern
     }
 
     if (!valid) return;
-    const int64_t slot = (int64_t)(own ? p.prefix_parts + part : part) * p.T * Hq + (int64_t)tok * Hq + hq;
+    const int64_t all = (int64_t)p.T * Hq, row = (int64_t)tok * Hq + hq;
     float l0, l1;
     half_wave_pair(l_run, l0, l1);
-    if (geo.hh == 0) {
-        p.part_ml[2 * slot] = m_run;
-        p.part_ml[2 * slot + 1] = l0 + l1;
+    const float l = l0 + l1;
+    // (a short request's rows have the P items' parts in front of their own)
+    const int before = stacked || rows >= 128 ? 0 : plan.prefix_parts;
+    if (!stacked && part == 0 && geo.hh == 0) p.row_parts[row] = before + parts == 1 ? 0 : before + parts;
+    if (!stacked && before + parts == 1) {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        uint16_t* og = p.o + tok * p.o_tok + hq * p.o_head;
+#pragma unroll
+        for (int db = 0; db < HD::kBlocks; ++db)
+#pragma unroll
+            for (int g4 = 0; g4 < 4; ++g4) {
+                typename Elem<E>::v4 x;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = (E)(oacc[db][4 * g4 + e] * inv);
+                *reinterpret_cast<typename Elem<E>::v4*>(og + 32 * db + 8 * g4 + 4 * geo.hh) = x;
+            }
+        return;
     }
+    const int64_t slot = (before + part) * all + row;
+    if (geo.hh == 0) *reinterpret_cast<f32x2*>(p.part_ml + 2 * slot) = f32x2{m_run, l};
+    if (n_tiles == 0) return;  // (nothing is read of a part whose sum is 0)
     float* oa = p.part_o + slot * D;
 #pragma unroll
     for (int db = 0; db < HD::kBlocks; ++db)
@@ -386,25 +507,41 @@ __global__ __launch_bounds__(256, SharedCfg<D>::kOcc) void fa_shared_prefix_kern
         }
 }
 
-// O = sum_s w_s o_s / sum_s w_s l_s,  w_s = exp2(m_s - max_s m_s): D / 4 lanes per row, rows of no request left alone.
+// O = sum_s w_s o_s / sum_s w_s l_s,  w_s = exp2(m_s - max_s m_s): D / 4 lanes per row, four parts in flight.  Rows of no
+// request and rows that are written already are left alone.
 template <typename E, int D>
 __global__ __launch_bounds__(256) void fa_shared_prefix_merge_kernel(const SharedPrefixParams p) {
-    constexpr int LPR = D / 4, RPB = 256 / LPR;
-    const int c = threadIdx.x % LPR, Hq = p.Hkv * p.g, parts = p.prefix_parts + p.own_parts;
+    constexpr int LPR = D / 4, RPB = 256 / LPR, U = 4;
+    const int c = threadIdx.x % LPR, Hq = p.Hkv * p.g;
     const int64_t rows = (int64_t)p.T * Hq, i = (int64_t)blockIdx.x * RPB + threadIdx.x / LPR;
     if (i >= rows) return;
     const int tok = (int)(i / Hq), hq = (int)(i - (int64_t)tok * Hq);
-    if (tok < clamp_int(p.q_start[0], 0, p.T) || tok >= clamp_int(p.q_start[p.B], 0, p.T)) return;
-    float m = -1e30f;
-    for (int s = 0; s < parts; ++s) m = max_nan(m, p.part_ml[2 * (s * rows + i)]);
+    const int first = p.q_start[0], last = p.q_start[p.B], parts = min(p.row_parts[i], p.max_prefix_parts + p.max_own_parts);
+    if (tok < first || tok >= last || parts <= 0) return;
+    const f32x2* ml = reinterpret_cast<const f32x2*>(p.part_ml) + i;
+    const float* po = p.part_o + i * D + 4 * c;
+    float m = -1e30f, l = 0.0f;
     f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    float l = 0.0f;
-    for (int s = 0; s < parts; ++s) {
-        const int64_t r = s * rows + i;
-        const float w = __builtin_amdgcn_exp2f(p.part_ml[2 * r] - m), ls = p.part_ml[2 * r + 1];
-        if (ls == 0.0f) continue;
-        l += w * ls;
-        acc += *reinterpret_cast<const f32x4*>(p.part_o + r * D + 4 * c) * w;
+    for (int s0 = 0; s0 < parts; s0 += U) {
+        f32x2 x[U];
+        f32x4 o[U];
+#pragma unroll
+        for (int s = 0; s < U; ++s) x[s] = ml[min(s0 + s, parts - 1) * rows];
+#pragma unroll
+        for (int s = 0; s < U; ++s) o[s] = *reinterpret_cast<const f32x4*>(po + min(s0 + s, parts - 1) * rows * D);
+        float mx = m;
+#pragma unroll
+        for (int s = 0; s < U; ++s) mx = max_nan(mx, x[s][0]);
+        const float a = __builtin_amdgcn_exp2f(m - mx);
+        m = mx, l *= a, acc *= a;
+#pragma unroll
+        for (int s = 0; s < U; ++s) {
+            const bool there = s0 + s < parts && x[s][1] != 0.0f;
+            const float w = there ? __builtin_amdgcn_exp2f(x[s][0] - m) : 0.0f;
+            l += w * x[s][1];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[e] += there ? w * o[s][e] : 0.0f;
+        }
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     typename Elem<E>::v4 out;

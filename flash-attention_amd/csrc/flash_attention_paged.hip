@@ -67,38 +67,34 @@ int check_cache(const fa_paged_cache* c) {
 }
 fa::CacheStrides strides_of(const int64_t (&s)[3]) { return {s[0], s[1], s[2]}; }
 
-// How a call divides its keys.  The chip wants a few workgroups per compute unit; every further part of a row costs
-// its state once out and once in.
-struct Parts {
-    int prefix_tiles, own_tiles;  // row tiles per K/V head
-    int prefix_parts, prefix_range, own_parts, own_range;
-    int parts() const { return prefix_parts + own_parts; }
-};
-constexpr int kMaxKeys = 1 << 30, kMaxParts = 64;
+constexpr int kMaxKeys = 1 << 30, kMaxParts = 64, kMaxBatch = 4096;
 
-Parts divide(int T, int B, int Hkv, int g, int prefix_len, int max_k_len, int cus) {
-    Parts d;
-    d.prefix_tiles = prefix_len > 0 ? (int)(((int64_t)T * g + 127) / 128) : 0;
-    d.own_tiles = fa::row_tiles_bound(T, B, g, 7);
+// What the host decides of a launch: the kernel divides the keys itself, from the lengths (SharedPlan); here are the
+// bounds that the workspace and the grid are made for.
+struct Bounds {
+    int slots;                            // workgroups resident at a time
+    int max_prefix_parts, max_own_parts;  // parts of one row's sum
+    int64_t blocks;                       // items of any lengths
+    int parts() const { return max_prefix_parts + max_own_parts; }
+};
+
+Bounds bounds_of(int T, int B, int Hkv, int g, int D, int prefix_len, int max_k_len, int cus) {
     auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
-    const int64_t prefix_steps = up(prefix_len, 64), own_steps = up(max_k_len, 64);
-    const int64_t total = Hkv * (d.prefix_tiles * prefix_steps + d.own_tiles * own_steps);
-    int64_t steps = up(total, 4 * (int64_t)cus);  // key tiles a workgroup walks
-    if (steps < 4) steps = 4;
-    auto cut = [&](int64_t all, int& parts, int& range) {
-        int64_t n = up(all, steps);
-        if (n > kMaxParts) n = kMaxParts;
-        if (n < 1) n = 1;
-        range = (int)(up(all, n) * 64);
-        parts = all > 0 ? (int)up(all * 64, range) : 1;
-        if (range == 0) range = 64;
-    };
-    cut(prefix_steps, d.prefix_parts, d.prefix_range);
-    cut(own_steps, d.own_parts, d.own_range);
-    if (prefix_len == 0) d.prefix_parts = 0;
+    auto within = [](int64_t x, int64_t lo, int64_t hi) { return (int)(x < lo ? lo : x > hi ? hi : x); };
+    const int64_t rows = (int64_t)T * g;
+    Bounds d;
+    d.slots = cus * (D == 256 ? 1 : 2);
+    // enough parts to fill the chip twice over from the prefix alone, or from a few requests' own keys; none shorter than 128 keys
+    d.max_prefix_parts = prefix_len > 0 ? within(up(2 * d.slots, up(rows, 128) * Hkv), 1, within(up(prefix_len, 128), 1, kMaxParts)) : 0;
+    d.max_own_parts = within(up(2 * d.slots, (int64_t)B * Hkv), 4, kMaxParts);
+    d.max_own_parts = within(up(max_k_len, 128), 1, d.max_own_parts);
+    const int64_t p_tiles = prefix_len > 0 ? fa::row_tiles(rows) : 0, r_tiles = fa::request_tiles_bound(rows, B);
+    d.blocks = std::min(Hkv * (p_tiles * d.max_prefix_parts + r_tiles * d.parts()), fa::blocks_bound(p_tiles, r_tiles, Hkv, d.slots));
     return d;
 }
-size_t workspace_of(const Parts& d, int T, int Hq, int D) { return (size_t)d.parts() * T * Hq * (D + 2) * sizeof(float); }
+size_t workspace_of(const Bounds& d, int T, int Hq, int D) {
+    return (size_t)T * Hq * ((size_t)d.parts() * (D + 2) * sizeof(float) + sizeof(int));
+}
 
 int check_shared(int T, int B, int Hq, int Hkv, int prefix_len, int max_k_len) {
     if (T < 0 || B < 0) return fail(FA_ERR_SHAPE, "fa_forward_shared_prefix: T and B must not be negative");
@@ -106,16 +102,16 @@ int check_shared(int T, int B, int Hq, int Hkv, int prefix_len, int max_k_len) {
         return fail(FA_ERR_SHAPE, "fa_forward_shared_prefix: the query heads must be a multiple of the cache's heads");
     if (prefix_len < 0 || prefix_len > kMaxKeys || max_k_len < 0 || max_k_len > kMaxKeys)
         return fail(FA_ERR_SEQLEN, "fa_forward_shared_prefix: lengths must be from 0 to 2^30");
+    if (B > kMaxBatch) return fail(FA_ERR_SHAPE, "fa_forward_shared_prefix: at most 4096 requests a call");
     if ((int64_t)T * Hq > 0x7fffffffLL / 64 || (int64_t)B * Hq > 0x7fffffffLL / 64)
         return fail(FA_ERR_SHAPE, "fa_forward_shared_prefix: T * Hq or B * Hq too large");
     return FA_OK;
 }
 
 template <typename E, int D>
-int launch_shared(const fa::SharedPrefixParams& p, const Parts& d, hipStream_t stream) {
-    const int64_t blocks = (int64_t)p.prefix_blocks + (int64_t)d.own_tiles * p.Hkv * d.own_parts;
-    if (blocks > 0x7fffffffLL) return fail(FA_ERR_SHAPE, "fa_forward_shared_prefix: grid size out of range");
-    hipLaunchKernelGGL((fa::fa_shared_prefix_kernel<E, D>), dim3((unsigned)blocks), dim3(256), 0, stream, p);
+int launch_shared(const fa::SharedPrefixParams& p, const Bounds& d, hipStream_t stream) {
+    if (d.blocks > 0x7fffffffLL) return fail(FA_ERR_SHAPE, "fa_forward_shared_prefix: grid size out of range");
+    hipLaunchKernelGGL((fa::fa_shared_prefix_kernel<E, D>), dim3((unsigned)d.blocks), dim3(256), 0, stream, p);
     if (int rc = hip_ok(hipGetLastError(), "fa_shared_prefix_kernel")) return rc;
     constexpr int rows = 256 / (D / 4);
     const int64_t merge = ((int64_t)p.T * p.Hkv * p.g + rows - 1) / rows;
@@ -188,7 +184,7 @@ size_t fa_shared_prefix_workspace(int T, int B, int Hq, int Hkv, int D, int pref
     if (T <= 0 || B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || prefix_len < 0 || prefix_len > kMaxKeys || max_k_len < 0 ||
         max_k_len > kMaxKeys)
         return 0;
-    return workspace_of(divide(T, B, Hkv, Hq / Hkv, prefix_len, max_k_len, fa_host::device_cus()), T, Hq, D);
+    return workspace_of(bounds_of(T, B, Hkv, Hq / Hkv, D, prefix_len, max_k_len, fa_host::device_cus()), T, Hq, D);
 }
 
 int fa_forward_shared_prefix(const uint16_t* dQ, int64_t q_tok, int64_t q_head, uint16_t* dO, int64_t o_tok, int64_t o_head,
@@ -211,7 +207,7 @@ int fa_forward_shared_prefix(const uint16_t* dQ, int64_t q_tok, int64_t q_head, 
         return fail(FA_ERR_POINTER, "fa_forward_shared_prefix: null pointer");
     if (!aligned16({dQ, dO}) || !whole_pieces({q_tok, q_head, o_tok, o_head}))
         return fail(FA_ERR_SHAPE, "fa_forward_shared_prefix: q and o must be 16-byte aligned, strides multiples of 8 elements");
-    const Parts d = divide(T, B, Hkv, Hq / Hkv, prefix_len, max_k_len, fa_host::device_cus());
+    const Bounds d = bounds_of(T, B, Hkv, Hq / Hkv, D, prefix_len, max_k_len, fa_host::device_cus());
     const size_t need = workspace_of(d, T, Hq, D);
     if (need > workspace_bytes || !workspace || !aligned16({workspace})) {
         char text[160];
@@ -227,14 +223,11 @@ int fa_forward_shared_prefix(const uint16_t* dQ, int64_t q_tok, int64_t q_head, 
     p.q_start = q_start, p.k_len = k_len;
     p.part_o = static_cast<float*>(workspace);
     p.part_ml = p.part_o + (size_t)d.parts() * T * Hq * D;
+    p.row_parts = reinterpret_cast<int*>(p.part_ml + (size_t)d.parts() * T * Hq * 2);
     p.T = T, p.B = B, p.Hkv = Hkv, p.g = Hq / Hkv, p.log2_page = log2_page, p.n_pages = cache->n_pages;
     p.prefix_len = prefix_len, p.table_width = table_width, p.causal = flags & FA_FLAG_CAUSAL;
     p.scale_log2e = scale * 1.44269504088896340736f;
-    p.prefix_parts = d.prefix_parts, p.prefix_range = d.prefix_range, p.own_parts = d.own_parts, p.own_range = d.own_range;
-    p.prefix_tiles = d.prefix_tiles, p.own_tiles = d.own_tiles;
-    const int64_t prefix_blocks = (int64_t)d.prefix_tiles * Hkv * d.prefix_parts;
-    if (prefix_blocks > 0x7fffffffLL) return fail(FA_ERR_SHAPE, "fa_forward_shared_prefix: grid size out of range");
-    p.prefix_blocks = (int)prefix_blocks;
+    p.slots = d.slots, p.max_prefix_parts = d.max_prefix_parts, p.max_own_parts = d.max_own_parts;
     hipStream_t stream = static_cast<hipStream_t>(stream_);
     return timed(stream, elapsed_ms, [&]() -> int {
         if (dtype == FA_DTYPE_FP16)

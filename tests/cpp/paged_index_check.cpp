@@ -50,21 +50,31 @@ int main() {
         const int b = owner_of(sum, (int)len.size(), x);
         need(sum[b] <= x && x < sum[b + 1], "owner_of", x, b);
     }
-    // row tiles: every request has room for its own, whatever the lengths; the bound covers them all
+    // workgroups of a launch: never more than the grid made from the bound, whatever the lengths
     std::srand(1);
     for (int trial = 0; trial < 20000; ++trial) {
-        const int B = 1 + std::rand() % 9, g = 1 + std::rand() % 20, log2r = std::rand() % 2 ? 7 : 5;
-        int start = 0, last = -1, T = 0;
-        std::vector<int> starts = {0};
-        for (int b = 0; b < B; ++b) starts.push_back(starts.back() + (std::rand() % 3 ? std::rand() % 4 : std::rand() % 300));
-        T = starts.back();
+        const int B = 1 + std::rand() % 40, heads = 1 + std::rand() % 9, g = 1 + std::rand() % 20, slots = std::rand() % 2 ? 512 : 256;
+        const int prefix = std::rand() % 3 ? std::rand() % 3000 : std::rand() % 3, least = 1 + std::rand() % 4;
+        const int most_prefix = 1 + std::rand() % 64, most_own = 1 + std::rand() % 64;
+        std::vector<int> rows(B), own(B);
+        long stacked = 0, total = 0;
+        float work = 0;
         for (int b = 0; b < B; ++b) {
-            start = first_row_tile(starts[b], b, g, log2r);
-            const int tiles = (int)(((long)(starts[b + 1] - starts[b]) * g + (1 << log2r) - 1) >> log2r);
-            need(start > last, "row tiles overlap", trial, b);
-            last = start + (tiles > 0 ? tiles : 1) - 1;
+            rows[b] = g * (std::rand() % 3 ? std::rand() % 4 : std::rand() % 300);
+            own[b] = std::rand() % 4 ? std::rand() % 40 : std::rand() % 5000;
+            total += rows[b];
+            if (rows[b] < 128) stacked += rows[b];
+            work += (float)row_tiles(rows[b]) * (own[b] + (rows[b] < 128 ? 0 : prefix));
         }
-        need(last < row_tiles_bound(T, B, g, log2r), "row tile bound", trial);
+        work += (float)row_tiles(stacked) * prefix;
+        const int steps = steps_for(work, heads, slots, least);
+        need(steps >= least, "steps", trial);
+        long items = prefix > 0 ? (long)heads * row_tiles(stacked) * parts_for(prefix, steps, most_prefix) : 0;
+        for (int b = 0; b < B; ++b)
+            items += (long)heads * row_tiles(rows[b]) *
+                     (rows[b] < 128 ? parts_for(own[b], steps, most_own) : parts_for(prefix + own[b], steps, most_prefix + most_own));
+        const long bound = blocks_bound(prefix > 0 ? row_tiles(total) : 0, request_tiles_bound(total, B), heads, slots);
+        need(items <= bound, "blocks", trial, items, bound);
     }
     std::printf("ok\n");
     return 0;
