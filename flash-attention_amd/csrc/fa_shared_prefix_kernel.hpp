@@ -50,6 +50,8 @@ struct Elem<_Float16> {
     typedef _Float16 v4 __attribute__((ext_vector_type(4)));
     static constexpr unsigned kExpMask = 0x7c00;
     static __device__ __forceinline__ f32x16 mfma(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ f32x4 mfma16(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ f32x4 mfma16(v4 a, v4 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x16f16(a, b, c, 0, 0, 0); }
 };
 template <>
 struct Elem<__bf16> {
@@ -57,35 +59,47 @@ struct Elem<__bf16> {
     typedef __bf16 v4 __attribute__((ext_vector_type(4)));
     static constexpr unsigned kExpMask = 0x7f80;
     static __device__ __forceinline__ f32x16 mfma(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ f32x4 mfma16(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ f32x4 mfma16(v4 a, v4 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(short4_t, a), __builtin_bit_cast(short4_t, b), c, 0, 0, 0);
+    }
 };
 
 // max that keeps NaN (v_maximum3_f32): a row that sees a NaN score is NaN, and no operand is canonicalised first.
 __device__ __forceinline__ float max_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
-// Infinities and NaN of a V fragment: taken out (returned fragment), and their places (kind 1 NaN, 2 +inf, 3 -inf) as ones.
-template <typename E>
-__device__ __forceinline__ typename Elem<E>::v8 finite_part(typename Elem<E>::v8 x, bool& special) {
-    u32x4 u = __builtin_bit_cast(u32x4, x);
+// Infinities and NaN of a V fragment (4 or 8 elements): taken out (returned fragment), and their places (kind 1 NaN, 2 +inf,
+// 3 -inf) as ones.
+template <typename E, typename V>
+__device__ __forceinline__ V finite_part(V x, bool& special) {
+    constexpr int W = sizeof(V) / 4;
+    typedef unsigned words __attribute__((ext_vector_type(W)));
+    words u = __builtin_bit_cast(words, x);
     constexpr unsigned m = Elem<E>::kExpMask;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < W; ++i) {
         if ((u[i] & m) == m) u[i] &= 0xffff0000u, special = true;
         if ((u[i] & (m << 16)) == m << 16) u[i] &= 0x0000ffffu, special = true;
     }
-    return __builtin_bit_cast(typename Elem<E>::v8, u);
+    return __builtin_bit_cast(V, u);
 }
-template <typename E>
-__device__ __forceinline__ typename Elem<E>::v8 special_part(typename Elem<E>::v8 x, int kind) {
-    const u32x4 u = __builtin_bit_cast(u32x4, x);
+template <typename E, typename V>
+__device__ __forceinline__ V special_part(V x, int kind) {
+    constexpr int W = sizeof(V) / 4;
+    typedef unsigned words __attribute__((ext_vector_type(W)));
+    const words u = __builtin_bit_cast(words, x);
     constexpr unsigned m = Elem<E>::kExpMask;
-    typename Elem<E>::v8 r;
+    V r;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 2 * W; ++i) {
         const unsigned h = (u[i / 2] >> (16 * (i & 1))) & 0xffffu, a = h & 0x7fffu;
         const int k = a > m ? 1 : a < m ? 0 : h == a ? 2 : 3;
         r[i] = (E)(k == kind ? 1.0f : 0.0f);
     }
     return r;
+}
+__device__ __forceinline__ float special_value(int kind) {
+    return __builtin_bit_cast(float, kind == 1 ? 0x7fc00000u : kind == 2 ? 0x7f800000u : 0xff800000u);
 }
 
 template <int D>
@@ -230,8 +244,289 @@ __device__ __forceinline__ void dma16(unsigned lds, const char* base, unsigned o
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds), "v"(off), "s"(base) : "memory");
 }
 
+// One workgroup's work: rows row0 .. of a request's `rows` (or of the stacked ones), K/V head `head`, key tiles u0 .. u0 +
+// n_tiles of the sequence of the prefix' tiles and the request's own.
+struct SharedItem {
+    int head, part, parts, before, row0, rows, u0, n_tiles, prefix_tiles, own_keys, n_tok;
+    bool stacked;
+    const int* own_table;
+};
+
+// Page of the 16-key group `group` of an item's range, -1 where there is none.
+template <int TK>
+__device__ __forceinline__ int page_of_group(const SharedPrefixParams& p, const SharedItem& it, int group, int end) {
+    constexpr int CPT = TK / 16;
+    const int u = it.u0 + group / CPT, own = u - it.prefix_tiles;
+    const int* table = own < 0 ? p.prefix_table : it.own_table;
+    const int j = ((own < 0 ? u : own) * TK + 16 * (group % CPT)) >> p.log2_page;
+    const int page = group < end && j < (own < 0 ? pages_for(p.prefix_len, p.log2_page) : p.table_width) ? table[j] : -1;
+    return page_ok(page, p.n_pages) ? page : -1;
+}
+
+// Where a row of the item lies in the workspace, once its sum of parts is known.
+__device__ __forceinline__ int64_t part_slot(const SharedPrefixParams& p, const SharedItem& it, int64_t row) {
+    return (int64_t)(it.before + it.part) * p.T * (p.Hkv * p.g) + row;
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// Up to 16 * RB rows: a single token's heads, or a few tokens'.  The work is bound by reading K and V, so each wave
+// takes a quarter of the item's keys for itself, 16 keys (a granule, on one page) at a time, through a ring of its own:
+// no barrier in the loop, and two granules and more per wave on their way.  S^T = K.Q^T is one 16 x 16 block per 16 rows
+// (v_mfma 16x16x32), whose registers are the B operand of O^T += V^T.P^T (16x16x16) as they are.  The four waves' sums are joined
+// through LDS at the end.
+// Bank conflicts: a K read takes 16 rows' 16 bytes of one column, a V read 8 rows' 32 bytes (half a wave at a time); the
+// chunks of a row are exchanged so that they fall on all 64 banks.
+template <typename E, int D, int RB>
+__device__ __forceinline__ void shared_few_rows(const SharedPrefixParams& p, const SharedItem& it, const int (&toks)[2], char* ring) {
+    using v8 = typename Elem<E>::v8;
+    using v4 = typename Elem<E>::v4;
+    constexpr int TK = SharedCfg<D>::kTk, CPT = TK / 16, kRow = 2 * D, kGran = 16 * kRow, CH = D / 8;
+    constexpr int N = SharedCfg<D>::kStages * 2 * TK * kRow / 4 / (2 * kGran);  // granules in a wave's ring
+    constexpr int NP = kGran / 1024, RPP = 1024 / kRow;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r16 = lane & 15, q4 = lane >> 4, Hq = p.Hkv * p.g, P1 = (1 << p.log2_page) - 1;
+    auto k_swz = [](int row) { return CH == 8 ? (row >> 1) & 7 : row & 15; };
+    auto v_swz = [](int row) { return CH == 8 ? (row & 6) : (row & 7) << 1; };
+
+    int limit[RB], hq[RB];
+    v8 qf[RB][D / 32];
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+        const int R = min(it.row0 + 16 * rb + r16, it.rows - 1), ti = R / p.g;
+        hq[rb] = it.head * p.g + (R - ti * p.g);
+        limit[rb] = p.causal ? min(it.own_keys - 1, it.own_keys - it.n_tok + ti) : it.own_keys - 1;
+        const uint16_t* qr = p.q + toks[rb] * p.q_tok + hq[rb] * p.q_head + q4 * 8;
+#pragma unroll
+        for (int ks = 0; ks < D / 32; ++ks) qf[rb][ks] = *reinterpret_cast<const v8*>(qr + ks * 32);
+    }
+
+    const int all = it.n_tiles * CPT, g0 = (int)((int64_t)all * wave / 4), n = (int)((int64_t)all * (wave + 1) / 4) - g0;
+    char* mine = ring + wave * N * 2 * kGran;
+    const unsigned lds = __builtin_amdgcn_readfirstlane((unsigned)(size_t)(__attribute__((address_space(3))) char*)mine);
+    const int d_rip = lane / CH, d_slot = lane % CH;
+    unsigned k_off[NP], v_off[NP];
+#pragma unroll
+    for (int j = 0; j < NP; ++j) {
+        const int row = RPP * j + d_rip;
+        k_off[j] = (unsigned)(row * (int)p.ks.row * 2) + (unsigned)((d_slot ^ k_swz(row)) << 4);
+        v_off[j] = (unsigned)(row * (int)p.vs.row * 2) + (unsigned)((d_slot ^ v_swz(row)) << 4);
+    }
+    const char* k_head = reinterpret_cast<const char*>(p.kc + it.head * p.ks.head);
+    const char* v_head = reinterpret_cast<const char*>(p.vc + it.head * p.vs.head);
+    int pages = page_of_group<TK>(p, it, g0 + lane, g0 + n), pages_next = -1;
+    if (n > 64) pages_next = page_of_group<TK>(p, it, g0 + 64 + lane, g0 + n);
+    int page_k = 0, row_k = 0;
+    auto send_k = [&](int i) {
+        if ((i & 63) == 0 && i > 0) {
+            pages = pages_next;
+            if (i + 64 < n) pages_next = page_of_group<TK>(p, it, g0 + i + 64 + lane, g0 + n);
+        }
+        const int g = g0 + i, u = it.u0 + g / CPT;
+        page_k = __builtin_amdgcn_readlane(pages, i & 63);
+        row_k = ((u < it.prefix_tiles ? u : u - it.prefix_tiles) * TK + 16 * (g % CPT)) & P1;
+        const char* base = k_head + 2 * ((int64_t)max(page_k, 0) * p.ks.page + (int64_t)row_k * p.ks.row);
+        const unsigned l = lds + (unsigned)(i % N) * 2 * kGran;
+#pragma unroll
+        for (int j = 0; j < NP; ++j) dma16(l + 1024u * j, base, k_off[j]);
+    };
+    auto send_v = [&](int i) {  // (right after send_k of the same granule, as far as pages go)
+        const char* base = v_head + 2 * ((int64_t)max(page_k, 0) * p.vs.page + (int64_t)row_k * p.vs.row);
+        const unsigned l = lds + (unsigned)(i % N) * 2 * kGran + kGran;
+#pragma unroll
+        for (int j = 0; j < NP; ++j) dma16(l + 1024u * j, base, v_off[j]);
+    };
+    uint64_t there = 0;  // bit j: granule i + j lies on a page
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        if (i < n) {
+            send_k(i);
+            send_v(i);
+            there |= (uint64_t)(page_k >= 0) << i;
+        }
+
+    f32x4 o[RB][D / 16];
+    float m_run[RB], l_run[RB];
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+        m_run[rb] = -1e30f, l_run[rb] = 0.0f;
+#pragma unroll
+        for (int db = 0; db < D / 16; ++db) o[rb][db] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    int k_rd[D / 32], v_rd;
+#pragma unroll
+    for (int ks = 0; ks < D / 32; ++ks) k_rd[ks] = r16 * kRow + (((4 * ks + q4) ^ k_swz(r16)) << 4);
+    const int v_row = 4 * q4 + (r16 >> 2);  // lane 4 q + pp of a group of 16 gives row q, 8 bytes pp
+    v_rd = v_row * kRow + 8 * (lane & 1);
+    const int v_ch = (lane >> 1) & 1, v_x = v_swz(v_row);
+    auto v_frag = [&](const char* vb, int db) -> v4 {
+        return __builtin_bit_cast(v4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                          (__attribute__((address_space(3))) short4_t*)(vb + v_rd + (((2 * db + v_ch) ^ v_x) << 4))));
+    };
+    auto max4 = [](f32x4 s) { return max_nan(max_nan(s[0], s[1]), max_nan(s[2], s[3])); };
+
+    for (int i = 0; i < n; ++i) {
+        const bool more = i + N < n;
+        const char* kb = mine + (i % N) * 2 * kGran;
+        const char* vb = kb + kGran;
+        if (more)
+            asm volatile("s_waitcnt vmcnt(%0)" : : "n"((2 * N - 1) * NP) : "memory");
+        else
+            wait_all_vmem();
+        f32x4 s[RB];
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) s[rb] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int ks = 0; ks < D / 32; ++ks) {
+            const v8 a = *reinterpret_cast<const v8*>(kb + k_rd[ks]);
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) s[rb] = Elem<E>::mfma16(a, qf[rb][ks], s[rb]);
+        }
+        if (more) {  // K's place is free: its reads have completed
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            send_k(i + N);
+        }
+        const int g = g0 + i, u = it.u0 + g / CPT, key = (u < it.prefix_tiles ? u : u - it.prefix_tiles) * TK + 16 * (g % CPT);
+        int lim[RB];
+        bool masked = !(there & 1);
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+            lim[rb] = (u < it.prefix_tiles ? p.prefix_len - 1 : limit[rb]) - key;
+            masked = masked || __any(lim[rb] < 15);
+        }
+        if (masked) {
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (4 * q4 + e > lim[rb] || !(there & 1)) s[rb][e] = -__builtin_inff();
+        }
+        v4 pf[RB];
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+            const float mx = max4(s[rb]) * p.scale_log2e;  // of this lane's four keys: the row's own is needed only when it moves
+            if (!__all(mx - m_run[rb] <= kRescaleSlack)) {
+                float a, b, m = mx;
+                half_wave_pair(m, a, b);
+                m = max_nan(a, b);
+                m = max_nan(m, __shfl_xor(m, 16));
+                const float m_new = max_nan(m_run[rb], m), alpha = __builtin_amdgcn_exp2f(m_run[rb] - m_new);
+                m_run[rb] = m_new;
+                l_run[rb] *= alpha;
+#pragma unroll
+                for (int db = 0; db < D / 16; ++db)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[rb][db][e] *= alpha;
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rb][e], p.scale_log2e, -m_run[rb]));
+                l_run[rb] += x;
+                pf[rb][e] = (E)x;
+            }
+        }
+        if (more)
+            asm volatile("s_waitcnt vmcnt(%0)" : : "n"((2 * N - 1) * NP) : "memory");
+        if (!masked) {
+#pragma unroll
+            for (int db = 0; db < D / 16; ++db) {
+                const v4 a = v_frag(vb, db);
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb) o[rb][db] = Elem<E>::mfma16(a, pf[rb], o[rb][db]);
+            }
+        } else {
+            bool special = false;
+#pragma unroll
+            for (int db = 0; db < D / 16; ++db) {
+                const v4 a = finite_part<E>(v_frag(vb, db), special);
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb) o[rb][db] = Elem<E>::mfma16(a, pf[rb], o[rb][db]);
+            }
+            if (__any(special)) {
+#pragma unroll 1
+                for (int kind = 1; kind <= 3; ++kind)
+#pragma unroll
+                    for (int rb = 0; rb < RB; ++rb) {
+                        v4 sees;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) sees[e] = (E)(4 * q4 + e <= lim[rb] && (there & 1) ? 1.0f : 0.0f);
+#pragma unroll
+                        for (int db = 0; db < D / 16; ++db) {
+                            const f32x4 c = Elem<E>::mfma16(special_part<E>(v_frag(vb, db), kind), sees, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                if (c[e] > 0.0f) o[rb][db][e] += special_value(kind);
+                        }
+                    }
+            }
+        }
+        there >>= 1;
+        if (more) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            send_v(i + N);
+            there |= (uint64_t)(page_k >= 0) << (N - 1);
+        }
+    }
+    wait_all_vmem();
+
+    // ---- the four waves' sums: 16 rows at a time through LDS, rows padded so that a store's 16 rows fall on all banks
+    constexpr int kOut = D + 4;  // floats
+    float* lo = reinterpret_cast<float*>(ring);
+    float* lml = lo + 4 * 16 * kOut;
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+        float a, b;
+        half_wave_pair(l_run[rb], a, b);
+        float l = a + b;
+        l += __shfl_xor(l, 16);
+        __syncthreads();  // (every wave is done with its ring, or with the rows before)
+        if (q4 == 0) {
+            lml[(wave * 16 + r16) * 2] = m_run[rb];
+            lml[(wave * 16 + r16) * 2 + 1] = l;
+        }
+#pragma unroll
+        for (int db = 0; db < D / 16; ++db) *reinterpret_cast<f32x4*>(lo + (wave * 16 + r16) * kOut + 16 * db + 4 * q4) = o[rb][db];
+        int* where = reinterpret_cast<int*>(lml + 128);  // token and head of each row
+        if (wave == 0 && q4 == 0) {
+            where[2 * r16] = toks[rb];
+            where[2 * r16 + 1] = hq[rb];
+        }
+        __syncthreads();
+        constexpr int C4 = D / 4;
+        for (int x = tid; x < 16 * C4; x += 256) {
+            const int row = x / C4, c = x % C4;
+            if (it.row0 + 16 * rb + row >= it.rows) continue;
+            float m = -1e30f, sum = 0.0f;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) m = max_nan(m, lml[(w * 16 + row) * 2]);
+            f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const float f = __builtin_amdgcn_exp2f(lml[(w * 16 + row) * 2] - m);
+                sum += f * lml[(w * 16 + row) * 2 + 1];
+                acc += *reinterpret_cast<const f32x4*>(lo + (w * 16 + row) * kOut + 4 * c) * f;
+            }
+            const int tok = where[2 * row], h = where[2 * row + 1];
+            const int64_t at = (int64_t)tok * Hq + h;
+            const int total = it.before + it.parts;
+            if (!it.stacked && it.part == 0 && c == 0) p.row_parts[at] = total == 1 ? 0 : total;
+            if (!it.stacked && total == 1) {
+                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                v4 y;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[e] = (E)(acc[e] * inv);
+                *reinterpret_cast<v4*>(p.o + tok * p.o_tok + h * p.o_head + 4 * c) = y;
+            } else {
+                const int64_t slot = part_slot(p, it, at);
+                if (c == 0) *reinterpret_cast<f32x2*>(p.part_ml + 2 * slot) = f32x2{m, sum};
+                *reinterpret_cast<f32x4*>(p.part_o + slot * D + 4 * c) = acc;
+            }
+        }
+    }
+}
+
+// Many rows: four waves of 32, key tiles shared through the ring.
 template <typename E, int D>
-__global__ __launch_bounds__(256, SharedCfg<D>::kOcc) void fa_shared_prefix_kernel(const SharedPrefixParams p) {
+__device__ __forceinline__ void shared_many_rows(const SharedPrefixParams& p, const SharedItem& it, int tok, char* ring) {
     using HD = HeadDim<D>;
     using CFG = SharedCfg<D>;
     using v8 = typename Elem<E>::v8;
@@ -240,60 +535,13 @@ __global__ __launch_bounds__(256, SharedCfg<D>::kOcc) void fa_shared_prefix_kern
     constexpr int RPP = 1024 / HD::kRow;             // rows per piece
     constexpr int RPW = RPP * PPW;                   // rows per wave and tile: 16 (D = 64) or 8, on one page
     constexpr int CPT = TK / 16;                     // 16-key groups per tile
-    __shared__ __attribute__((aligned(1024))) char ring[ST * kStage];
-
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const LaneGeomD<D> geo = make_lane_geom_d<D>(lane);
     const int P1 = (1 << p.log2_page) - 1;  // (row in a page)
-
-    // ---- which rows against which keys: rows row0 .. of a request's `rows` (or of the stacked ones) against key tiles
-    //      u0 .. of the sequence of the prefix' tiles and the request's own
-    SharedPlan plan;
-    int head, part, parts, row0, rows, u0, n_tiles, own_keys = 0, n_tok = 0, tok;
-    bool stacked;
-    const int* own_table = nullptr;
-    const int R_off = wave * 32 + geo.r;
-    {
-        int* stacked_start = reinterpret_cast<int*>(ring);  // (free until the first transfer)
-        int* item_start = stacked_start + p.B;
-        __shared__ int tmp[4];
-        const int x = (int)blockIdx.x;
-        if (x >= shared_plan<TK>(p, plan, stacked_start, item_start, tmp)) return;
-        int unit, tile, u1;
-        stacked = x < plan.p_items;
-        if (stacked) {
-            parts = plan.prefix_parts;
-            unit_and_tile(x, p.Hkv * parts, (plan.stacked + 127) >> 7, unit, tile);
-            head = unit / parts, part = unit - head * parts;
-            row0 = tile * 128, rows = plan.stacked;
-            u0 = (int)((int64_t)plan.prefix_tiles * part / parts);
-            u1 = (int)((int64_t)plan.prefix_tiles * (part + 1) / parts);
-            const int t = min(row0 + R_off, rows - 1) / p.g;  // stacked token
-            const int b = owner_of(stacked_start, p.B, t);
-            tok = clamp_int(p.q_start[b], 0, p.T) + t - stacked_start[b];
-        } else {
-            const int b = last_at_most(item_start, p.B, x);
-            const SharedRequest r = shared_request(p, b);
-            int tiles;
-            request_items<TK>(p, plan, r, tiles, parts);
-            unit_and_tile(x - item_start[b], p.Hkv * parts, tiles, unit, tile);
-            head = unit / parts, part = unit - head * parts;
-            row0 = tile * 128, rows = r.n * p.g, n_tok = r.n;
-            own_keys = r.keys;
-            own_table = p.block_table + b * p.table_stride;
-            tok = r.tok0 + min(row0 + R_off, rows - 1) / p.g;
-            // no row of the tile sees further than its last one
-            const int last_ti = (min(row0 + 128, rows) - 1) / p.g, see = p.causal ? min(r.keys, r.keys - r.n + last_ti + 1) : r.keys;
-            const int first = rows >= 128 ? 0 : plan.prefix_tiles, n = plan.prefix_tiles + (max(see, 0) + TK - 1) / TK - first;
-            u0 = first + (int)((int64_t)n * part / parts);
-            u1 = first + (int)((int64_t)n * (part + 1) / parts);
-        }
-        n_tiles = u1 - u0;
-        __syncthreads();  // (the tables above have been read)
-    }
+    const int R_off = wave * 32 + geo.r, head = it.head, row0 = it.row0, rows = it.rows, u0 = it.u0, n_tiles = it.n_tiles;
     const bool valid = row0 + R_off < rows, wave_valid = row0 + wave * 32 < rows;
     const int R = min(row0 + R_off, rows - 1), ti = R / p.g, hq = head * p.g + (R - ti * p.g), Hq = p.Hkv * p.g;
-    const int own_limit = p.causal ? min(own_keys - 1, own_keys - n_tok + ti) : own_keys - 1;  // the last own key this row sees
+    const int own_limit = p.causal ? min(it.own_keys - 1, it.own_keys - it.n_tok + ti) : it.own_keys - 1;  // the last own key this row sees
 
     // ---- transfers: this wave moves rows RPW * wave .. of each tile.  They lie on one page, whose number is uniform: lane L
     //      holds the entry of the 16-key group group0 + L of the range, 64 groups at a time (the next 64 are loaded one
@@ -309,14 +557,7 @@ __global__ __launch_bounds__(256, SharedCfg<D>::kOcc) void fa_shared_prefix_kern
     }
     const char* k_head = reinterpret_cast<const char*>(p.kc + head * p.ks.head);
     const char* v_head = reinterpret_cast<const char*>(p.vc + head * p.vs.head);
-    const int own_entries = p.table_width, prefix_entries = pages_for(p.prefix_len, p.log2_page);
-    auto load_pages = [&](int group) -> int {  // -1: no page
-        const int i = group + lane, u = u0 + i / CPT, key = (u < plan.prefix_tiles ? u : u - plan.prefix_tiles) * TK + 16 * (i % CPT);
-        const int* table = u < plan.prefix_tiles ? p.prefix_table : own_table;
-        const int j = key >> p.log2_page;
-        const int page = i < n_tiles * CPT && j < (u < plan.prefix_tiles ? prefix_entries : own_entries) ? table[j] : -1;
-        return page_ok(page, p.n_pages) ? page : -1;
-    };
+    auto load_pages = [&](int group) -> int { return page_of_group<TK>(p, it, group + lane, n_tiles * CPT); };
     int pages = 0, pages_next = 0;
     unsigned on_page = 0;  // CPT bits per tile sent for and not yet computed: the groups that lie on a page
     auto send = [&](int t) {
@@ -328,7 +569,7 @@ __global__ __launch_bounds__(256, SharedCfg<D>::kOcc) void fa_shared_prefix_kern
         on_page |= ((unsigned)(__ballot(pages >= 0) >> (g0 & 63)) & ((1u << CPT) - 1)) << (CPT * (ST - 1));
         // (a group on no page is fetched from page 0: its scores are masked)
         const int page = max(__builtin_amdgcn_readlane(pages, (g0 + wave * RPW / 16) & 63), 0);
-        const int u = u0 + t, row = ((u < plan.prefix_tiles ? u : u - plan.prefix_tiles) * TK + wave * RPW) & P1;
+        const int u = u0 + t, row = ((u < it.prefix_tiles ? u : u - it.prefix_tiles) * TK + wave * RPW) & P1;
         const char* kb = k_head + 2 * ((int64_t)page * p.ks.page + (int64_t)row * p.ks.row);
         const char* vb = v_head + 2 * ((int64_t)page * p.vs.page + (int64_t)row * p.vs.row);
         const unsigned l = ring_lds + (unsigned)(t % ST) * kStage + (unsigned)(PPW * wave) * 1024u;
@@ -373,7 +614,7 @@ __global__ __launch_bounds__(256, SharedCfg<D>::kOcc) void fa_shared_prefix_kern
         on_page >>= CPT;
         const int u = u0 + t;
         // the last key of this tile that the row sees; a wave whose rows see none of it passes it by
-        const int lim = u < plan.prefix_tiles ? p.prefix_len - 1 - u * TK : own_limit - (u - plan.prefix_tiles) * TK;
+        const int lim = u < it.prefix_tiles ? p.prefix_len - 1 - u * TK : own_limit - (u - it.prefix_tiles) * TK;
         if (wave_valid && __any(lim >= 0)) {
             const char* kb = ring + (t % ST) * kStage;
             const char* vb = kb + kTile;
@@ -447,7 +688,6 @@ __global__ __launch_bounds__(256, SharedCfg<D>::kOcc) void fa_shared_prefix_kern
                         }
 #pragma unroll 1
                     for (int kind = 1; kind <= 3; ++kind) {
-                        const unsigned bits = kind == 1 ? 0x7fc00000u : kind == 2 ? 0x7f800000u : 0xff800000u;
 #pragma unroll
                         for (int db = 0; db < HD::kBlocks; ++db) {
                             f32x16 n;
@@ -458,7 +698,7 @@ __global__ __launch_bounds__(256, SharedCfg<D>::kOcc) void fa_shared_prefix_kern
                                 n = Elem<E>::mfma(special_part<E>(v_frag(vb, kk, db), kind), sees[kk], n);
 #pragma unroll
                             for (int e = 0; e < 16; ++e)
-                                if (n[e] > 0.0f) oacc[db][e] += __builtin_bit_cast(float, bits);
+                                if (n[e] > 0.0f) oacc[db][e] += special_value(kind);
                         }
                     }
                 }
@@ -473,14 +713,13 @@ __global__ __launch_bounds__(256, SharedCfg<D>::kOcc) void fa_shared_prefix_kern
     }
 
     if (!valid) return;
-    const int64_t all = (int64_t)p.T * Hq, row = (int64_t)tok * Hq + hq;
+    const int64_t row = (int64_t)tok * Hq + hq;
     float l0, l1;
     half_wave_pair(l_run, l0, l1);
     const float l = l0 + l1;
-    // (a short request's rows have the P items' parts in front of their own)
-    const int before = stacked || rows >= 128 ? 0 : plan.prefix_parts;
-    if (!stacked && part == 0 && geo.hh == 0) p.row_parts[row] = before + parts == 1 ? 0 : before + parts;
-    if (!stacked && before + parts == 1) {
+    const int total = it.before + it.parts;
+    if (!it.stacked && it.part == 0 && geo.hh == 0) p.row_parts[row] = total == 1 ? 0 : total;
+    if (!it.stacked && total == 1) {
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         uint16_t* og = p.o + tok * p.o_tok + hq * p.o_head;
 #pragma unroll
@@ -494,7 +733,7 @@ __global__ __launch_bounds__(256, SharedCfg<D>::kOcc) void fa_shared_prefix_kern
             }
         return;
     }
-    const int64_t slot = (before + part) * all + row;
+    const int64_t slot = part_slot(p, it, row);
     if (geo.hh == 0) *reinterpret_cast<f32x2*>(p.part_ml + 2 * slot) = f32x2{m_run, l};
     if (n_tiles == 0) return;  // (nothing is read of a part whose sum is 0)
     float* oa = p.part_o + slot * D;
@@ -505,6 +744,63 @@ __global__ __launch_bounds__(256, SharedCfg<D>::kOcc) void fa_shared_prefix_kern
             const f32x4 x = {oacc[db][4 * g4], oacc[db][4 * g4 + 1], oacc[db][4 * g4 + 2], oacc[db][4 * g4 + 3]};
             *reinterpret_cast<f32x4*>(oa + 32 * db + 8 * g4 + 4 * geo.hh) = x;
         }
+}
+
+template <typename E, int D>
+__global__ __launch_bounds__(256, SharedCfg<D>::kOcc) void fa_shared_prefix_kernel(const SharedPrefixParams p) {
+    constexpr int TK = SharedCfg<D>::kTk;
+    __shared__ __attribute__((aligned(1024))) char ring[SharedCfg<D>::kStages * 2 * TK * 2 * D];
+    SharedItem it;
+    int toks[2];  // of this lane's rows: 32 wave + (lane & 31), or, of few rows, (lane & 15) and 16 + (lane & 15)
+    bool few;
+    {
+        int* stacked_start = reinterpret_cast<int*>(ring);  // (free until the first transfer)
+        int* item_start = stacked_start + p.B;
+        __shared__ int tmp[4];
+        SharedPlan plan;
+        const int x = (int)blockIdx.x, lane = threadIdx.x & 63;
+        if (x >= shared_plan<TK>(p, plan, stacked_start, item_start, tmp)) return;
+        it.prefix_tiles = plan.prefix_tiles;
+        it.stacked = x < plan.p_items;
+        int unit, tile, tiles, b = 0, tok0 = 0;
+        it.own_keys = it.n_tok = 0;
+        it.own_table = nullptr;
+        if (it.stacked) {
+            it.rows = plan.stacked, it.parts = plan.prefix_parts, tiles = row_tiles(plan.stacked);
+        } else {
+            b = last_at_most(item_start, p.B, x);
+            const SharedRequest r = shared_request(p, b);
+            request_items<TK>(p, plan, r, tiles, it.parts);
+            it.rows = r.n * p.g, it.n_tok = r.n, it.own_keys = r.keys, tok0 = r.tok0;
+            it.own_table = p.block_table + b * p.table_stride;
+        }
+        unit_and_tile(x - (it.stacked ? 0 : item_start[b]), p.Hkv * it.parts, tiles, unit, tile);
+        it.head = unit / it.parts, it.part = unit - it.head * it.parts, it.row0 = tile * kRowTile;
+        // the key tiles of this row tile: no row of it sees further than its last one
+        const int end = min(it.row0 + kRowTile, it.rows), short_ = it.rows < kRowTile;
+        const int see = p.causal ? min(it.own_keys, it.own_keys - it.n_tok + (end - 1) / p.g + 1) : it.own_keys;
+        const int first = it.stacked || !short_ ? 0 : plan.prefix_tiles;
+        const int last = it.stacked ? plan.prefix_tiles : plan.prefix_tiles + (max(see, 0) + TK - 1) / TK;
+        it.before = first > 0 ? plan.prefix_parts : 0;  // (parts that P items add in front of this item's)
+        it.u0 = first + (int)((int64_t)(last - first) * it.part / it.parts);
+        it.n_tiles = first + (int)((int64_t)(last - first) * (it.part + 1) / it.parts) - it.u0;
+        few = end - it.row0 <= 32;
+        auto token = [&](int off) -> int {
+            const int t = min(it.row0 + off, it.rows - 1) / p.g;
+            if (!it.stacked) return tok0 + t;
+            const int o = owner_of(stacked_start, p.B, t);
+            return clamp_int(p.q_start[o], 0, p.T) + t - stacked_start[o];
+        };
+        toks[0] = token(few ? lane & 15 : (int)(threadIdx.x >> 6) * 32 + (lane & 31));
+        toks[1] = few ? token(16 + (lane & 15)) : toks[0];
+        __syncthreads();  // (the tables above have been read)
+    }
+    if (!few)
+        shared_many_rows<E, D>(p, it, toks[0], ring);
+    else if (min(it.rows - it.row0, kRowTile) <= 16)
+        shared_few_rows<E, D, 1>(p, it, toks, ring);
+    else
+        shared_few_rows<E, D, 2>(p, it, toks, ring);
 }
 
 // O = sum_s w_s o_s / sum_s w_s l_s,  w_s = exp2(m_s - max_s m_s): D / 4 lanes per row, four parts in flight.  Rows of no
