@@ -82,34 +82,6 @@ __device__ __forceinline__ void mfma_vv(f32x16& d, const half8& a, const half8& 
     asm volatile("v_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+v"(d) : "v"(a), "v"(b));
 }
 
-// Makes the kernel descriptor allocate a[0:31] only (D = 64: the whole accumulator).  With several waves per SIMD a
-// wave's architectural and accumulator registers come out of one budget: 128 + 32 lets three workgroups share a CU.
-__device__ __forceinline__ void acc_reserve32() {
-    asm volatile("" : : : "a0", "a1", "a2", "a3", "a4", "a5", "a6", "a7", "a8", "a9", "a10", "a11", "a12", "a13", "a14", "a15",
-                 "a16", "a17", "a18", "a19", "a20", "a21", "a22", "a23", "a24", "a25", "a26", "a27", "a28", "a29", "a30", "a31");
-}
-__device__ __forceinline__ void acc_reserve64() {
-    asm volatile("" : : : "a0", "a1", "a2", "a3", "a4", "a5", "a6", "a7", "a8", "a9", "a10", "a11", "a12", "a13", "a14", "a15",
-                 "a16", "a17", "a18", "a19", "a20", "a21", "a22", "a23", "a24", "a25", "a26", "a27", "a28", "a29", "a30", "a31",
-                 "a32", "a33", "a34", "a35", "a36", "a37", "a38", "a39", "a40", "a41", "a42", "a43", "a44", "a45", "a46", "a47",
-                 "a48", "a49", "a50", "a51", "a52", "a53", "a54", "a55", "a56", "a57", "a58", "a59", "a60", "a61", "a62", "a63");
-}
-// a[LO : LO+15] = 0 through the matrix pipe; a[BASE : BASE+N-1] *= alpha through the vector ALU (rare: the rescale).
-template <int LO>
-__device__ __forceinline__ void acc_zero16() {
-    half8 z = {};
-    asm volatile("s_nop 3" : "+v"(z));  // wait states between the vector writes of z and the MFMA reading it
-    asm volatile("v_mfma_f32_32x32x16_f16 a[%1:%2], %0, %0, 0" : : "v"(z), "n"(LO), "n"(LO + 15));
-}
-template <int BASE, int N>
-__device__ __forceinline__ void acc_scale_n(float alpha) {
-    acc_fence();
-    static_for<N>([&](auto ic) {
-        constexpr int i = decltype(ic)::value;
-        acc_put<BASE + i>(acc_get<BASE + i>() * alpha);
-    });
-}
-
 // Scores of one tile, nothing beside them (the prologue): S^T = K.Q^T for KB key blocks, D / 16 k-steps.
 template <int D, int KB>
 __device__ __forceinline__ void hd_scores(const char* kb, const LaneGeomD<D>& g, const half8 (&qf)[HeadDim<D>::kSteps],

@@ -48,6 +48,7 @@
 #include <utility>
 
 #include "fa_fwd_ring_kernel.hpp"
+#include "fa_owned_acc.hpp"
 
 namespace fa {
 
@@ -137,18 +138,6 @@ __device__ __forceinline__ void vbuf_read(unsigned addr) {
                  : "memory");
 }
 __device__ __forceinline__ void lds_wait_all() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
-// Wait states between the last MFMA on an accumulator and a v_accvgpr_read of it.
-__device__ __forceinline__ void acc_fence() { asm volatile("s_nop 15\n\ts_nop 3"); }
-template <int R>
-__device__ __forceinline__ float acc_get() {
-    float x;
-    asm volatile("v_accvgpr_read_b32 %0, a[%1]" : "=v"(x) : "n"(R));
-    return x;
-}
-template <int R>
-__device__ __forceinline__ void acc_put(float x) {
-    asm volatile("v_accvgpr_write_b32 a[%1], %0" : : "v"(x), "n"(R));
-}
 template <int R>
 __device__ __forceinline__ void acc_put_u32(unsigned x) {
     asm volatile("v_accvgpr_write_b32 a[%1], %0" : : "v"(x), "n"(R));

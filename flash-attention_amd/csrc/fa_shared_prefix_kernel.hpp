@@ -17,6 +17,7 @@
 #pragma once
 #include "fa_fwd_general_kernel.hpp"
 #include "fa_fwd_ring_kernel.hpp"  // wait_all_vmem
+#include "fa_owned_acc.hpp"
 #include "fa_paged_index.hpp"
 
 namespace fa {
@@ -52,6 +53,10 @@ struct Elem<_Float16> {
     static __device__ __forceinline__ f32x16 mfma(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
     static __device__ __forceinline__ f32x4 mfma16(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
     static __device__ __forceinline__ f32x4 mfma16(v4 a, v4 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x16f16(a, b, c, 0, 0, 0); }
+    template <int LO>  // a[LO : LO + 15] += a.b
+    static __device__ __forceinline__ void mfma_owned(v8 a, v8 b) {
+        asm volatile("v_mfma_f32_32x32x16_f16 a[%2:%3], %0, %1, a[%2:%3]" : : "v"(a), "v"(b), "n"(LO), "n"(LO + 15));
+    }
 };
 template <>
 struct Elem<__bf16> {
@@ -62,6 +67,10 @@ struct Elem<__bf16> {
     static __device__ __forceinline__ f32x4 mfma16(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
     static __device__ __forceinline__ f32x4 mfma16(v4 a, v4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(short4_t, a), __builtin_bit_cast(short4_t, b), c, 0, 0, 0);
+    }
+    template <int LO>
+    static __device__ __forceinline__ void mfma_owned(v8 a, v8 b) {
+        asm volatile("v_mfma_f32_32x32x16_bf16 a[%2:%3], %0, %1, a[%2:%3]" : : "v"(a), "v"(b), "n"(LO), "n"(LO + 15));
     }
 };
 
@@ -106,15 +115,15 @@ template <int D>
 struct SharedCfg;
 template <>
 struct SharedCfg<64> {
-    static constexpr int kTk = 64, kStages = 4, kOcc = 2;  // 16 KiB a stage
+    static constexpr int kTk = 64, kStages = 4, kFewBlocks = 2;  // 16 KiB a stage
 };
 template <>
 struct SharedCfg<128> {
-    static constexpr int kTk = 32, kStages = 4, kOcc = 2;  // 16 KiB
+    static constexpr int kTk = 32, kStages = 4, kFewBlocks = 1;  // 16 KiB
 };
 template <>
 struct SharedCfg<256> {
-    static constexpr int kTk = 32, kStages = 4, kOcc = 1;  // 32 KiB
+    static constexpr int kTk = 32, kStages = 4, kFewBlocks = 1;  // 32 KiB
 };
 
 // The division of a launch into workgroups, from the requests' lengths; every workgroup computes it for itself.
@@ -362,8 +371,13 @@ __device__ __forceinline__ void shared_few_rows(const SharedPrefixParams& p, con
         return __builtin_bit_cast(v4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                                           (__attribute__((address_space(3))) short4_t*)(vb + v_rd + (((2 * db + v_ch) ^ v_x) << 4))));
     };
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb)  // (waited for here: see shared_many_rows)
+#pragma unroll
+        for (int ks = 0; ks < D / 32; ++ks) asm volatile("" : "+v"(qf[rb][ks]));
     auto max4 = [](f32x4 s) { return max_nan(max_nan(s[0], s[1]), max_nan(s[2], s[3])); };
 
+    int specials = 0;  // masked granules held infinities or NaN
     for (int i = 0; i < n; ++i) {
         const bool more = i + N < n;
         const char* kb = mine + (i % N) * 2 * kGran;
@@ -387,12 +401,13 @@ __device__ __forceinline__ void shared_few_rows(const SharedPrefixParams& p, con
         }
         const int g = g0 + i, u = it.u0 + g / CPT, key = (u < it.prefix_tiles ? u : u - it.prefix_tiles) * TK + 16 * (g % CPT);
         int lim[RB];
-        bool masked = !(there & 1);
+        bool any = !(there & 1);
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
             lim[rb] = (u < it.prefix_tiles ? p.prefix_len - 1 : limit[rb]) - key;
-            masked = masked || __any(lim[rb] < 15);
+            any = any || __any(lim[rb] < 15);
         }
+        const int masked = __builtin_amdgcn_readfirstlane((int)any);
         if (masked) {
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb)
@@ -441,23 +456,7 @@ __device__ __forceinline__ void shared_few_rows(const SharedPrefixParams& p, con
 #pragma unroll
                 for (int rb = 0; rb < RB; ++rb) o[rb][db] = Elem<E>::mfma16(a, pf[rb], o[rb][db]);
             }
-            if (__any(special)) {
-#pragma unroll 1
-                for (int kind = 1; kind <= 3; ++kind)
-#pragma unroll
-                    for (int rb = 0; rb < RB; ++rb) {
-                        v4 sees;
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) sees[e] = (E)(4 * q4 + e <= lim[rb] && (there & 1) ? 1.0f : 0.0f);
-#pragma unroll
-                        for (int db = 0; db < D / 16; ++db) {
-                            const f32x4 c = Elem<E>::mfma16(special_part<E>(v_frag(vb, db), kind), sees, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
-#pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                if (c[e] > 0.0f) o[rb][db][e] += special_value(kind);
-                        }
-                    }
-            }
+            specials |= __builtin_amdgcn_readfirstlane((int)__any(special));
         }
         there >>= 1;
         if (more) {
@@ -467,6 +466,40 @@ __device__ __forceinline__ void shared_few_rows(const SharedPrefixParams& p, con
         }
     }
     wait_all_vmem();
+    if (__builtin_expect(specials != 0, 0)) {
+        // the values taken out of masked granules, to the rows that do see them: those granules once more, one at a time
+#pragma unroll 1
+        for (int i = 0; i < n; ++i) {
+            const int g = g0 + i, u = it.u0 + g / CPT, key = (u < it.prefix_tiles ? u : u - it.prefix_tiles) * TK + 16 * (g % CPT);
+            const int page = __builtin_amdgcn_readfirstlane(page_of_group<TK>(p, it, g, g0 + n));
+            const int pre = u < it.prefix_tiles;
+            bool any = false;
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) any = any || __any((pre ? p.prefix_len - 1 : limit[rb]) - key < 15);
+            if (page < 0 || !any) continue;
+            const char* base = v_head + 2 * ((int64_t)page * p.vs.page + (int64_t)(key & P1) * p.vs.row);
+#pragma unroll
+            for (int j = 0; j < NP; ++j) dma16(lds + 1024u * j, base, v_off[j]);
+            wait_all_vmem();
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) {
+                v4 sees;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sees[e] = (E)(4 * q4 + e <= (pre ? p.prefix_len - 1 : limit[rb]) - key ? 1.0f : 0.0f);
+#pragma unroll
+                for (int db = 0; db < D / 16; ++db) {
+                    const v4 f = v_frag(mine, db);
+#pragma unroll
+                    for (int kind = 1; kind <= 3; ++kind) {
+                        const f32x4 c = Elem<E>::mfma16(special_part<E>(f, kind), sees, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[rb][db][e] += c[e] > 0.0f ? special_value(kind) : 0.0f;
+                    }
+                }
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        }
+    }
 
     // ---- the four waves' sums: 16 rows at a time through LDS, rows padded so that a store's 16 rows fall on all banks
     constexpr int kOut = D + 4;  // floats
@@ -560,7 +593,11 @@ __device__ __forceinline__ void shared_many_rows(const SharedPrefixParams& p, co
     auto load_pages = [&](int group) -> int { return page_of_group<TK>(p, it, group + lane, n_tiles * CPT); };
     int pages = 0, pages_next = 0;
     unsigned on_page = 0;  // CPT bits per tile sent for and not yet computed: the groups that lie on a page
-    auto send = [&](int t) {
+    struct Transfer {
+        const char *k, *v;
+        unsigned lds;
+    };
+    auto transfer = [&](int t) -> Transfer {
         const int g0 = t * CPT;
         if ((g0 & 63) == 0) {
             pages = t == 0 ? load_pages(0) : pages_next;
@@ -570,13 +607,20 @@ __device__ __forceinline__ void shared_many_rows(const SharedPrefixParams& p, co
         // (a group on no page is fetched from page 0: its scores are masked)
         const int page = max(__builtin_amdgcn_readlane(pages, (g0 + wave * RPW / 16) & 63), 0);
         const int u = u0 + t, row = ((u < it.prefix_tiles ? u : u - it.prefix_tiles) * TK + wave * RPW) & P1;
-        const char* kb = k_head + 2 * ((int64_t)page * p.ks.page + (int64_t)row * p.ks.row);
-        const char* vb = v_head + 2 * ((int64_t)page * p.vs.page + (int64_t)row * p.vs.row);
-        const unsigned l = ring_lds + (unsigned)(t % ST) * kStage + (unsigned)(PPW * wave) * 1024u;
-#pragma unroll
-        for (int j = 0; j < PPW; ++j) dma16(l + 1024u * j, kb, k_off[j]);
-#pragma unroll
-        for (int j = 0; j < PPW; ++j) dma16(l + kTile + 1024u * j, vb, v_off[j]);
+        return {k_head + 2 * ((int64_t)page * p.ks.page + (int64_t)row * p.ks.row),
+                v_head + 2 * ((int64_t)page * p.vs.page + (int64_t)row * p.vs.row),
+                ring_lds + (unsigned)(t % ST) * kStage + (unsigned)(PPW * wave) * 1024u};
+    };
+    auto send_piece = [&](const Transfer& tr, auto jc) {
+        constexpr int j = decltype(jc)::value;
+        if constexpr (j < PPW)
+            dma16(tr.lds + 1024u * j, tr.k, k_off[j]);
+        else
+            dma16(tr.lds + kTile + 1024u * (j - PPW), tr.v, v_off[j - PPW]);
+    };
+    auto send = [&](int t) {
+        const Transfer tr = transfer(t);
+        static_for<2 * PPW>([&](auto ic) { send_piece(tr, ic); });
     };
 
 #pragma unroll
@@ -592,124 +636,230 @@ __device__ __forceinline__ void shared_many_rows(const SharedPrefixParams& p, co
         for (int ks = 0; ks < HD::kSteps; ++ks) qf[ks] = *reinterpret_cast<const v8*>(qr + ks * 16);
     }
 
-    f32x16 oacc[HD::kBlocks];
+    f32x16 s_cur[KB], s_next[KB];
     float m_run = -1e30f, l_run = 0.0f;
-#pragma unroll
-    for (int db = 0; db < HD::kBlocks; ++db)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) oacc[db][e] = 0.0f;
+    const float c = p.scale_log2e;
 
+    auto k_frag = [&](const char* kb, int i) -> v8 { return *reinterpret_cast<const v8*>(kb + geo.k_rd[i / KB] + (i % KB) * 32 * HD::kRow); };
     auto v_frag = [&](const char* vb, int kk, int db) -> v8 {
         const char* a0 = vb + geo.v_rd[db] + kk * 16 * HD::kRow;
         const short4_t t0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t*)(a0));
         const short4_t t1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t*)(a0 + 8 * HD::kRow));
         return __builtin_bit_cast(v8, __builtin_shufflevector(t0, t1, 0, 1, 2, 3, 4, 5, 6, 7));
     };
+    // the last key of tile t that the row sees, counted from the tile's first; whether the tile needs the mask
+    auto limit_of = [&](int t) -> int {
+        const int u = u0 + t, own = u - it.prefix_tiles;
+        return (own < 0 ? p.prefix_len - 1 : own_limit) - (own < 0 ? u : own) * TK;
+    };
+    constexpr unsigned kAllGroups = (1u << CPT) - 1;
+    auto needs_mask = [&](int lim, unsigned groups) -> int {
+        return __builtin_amdgcn_readfirstlane((int)(__any(lim < TK - 1) || groups != kAllGroups));
+    };
+    auto mask_scores = [&](f32x16 (&s)[KB], int lim, unsigned groups) {
+#pragma unroll
+        for (int b = 0; b < KB; ++b)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int k = 32 * b + 8 * (e >> 2) + (e & 3);
+                if (k + 4 * geo.hh > lim || !((groups >> (k >> 4)) & 1)) s[b][e] = -__builtin_inff();
+            }
+    };
+    auto lane_max = [&](const f32x16 (&s)[KB]) -> float {
+        float m = max_nan(s[0][0], s[0][1]);
+#pragma unroll
+        for (int b = 0; b < KB; ++b)
+#pragma unroll
+            for (int e = b == 0 ? 2 : 0; e < 16; e += 2) m = max_nan(max_nan(m, s[b][e]), s[b][e + 1]);
+        return m * c;
+    };
+    // the reference moves only when some row's score passes it by more than kRescaleSlack: this lane's half of the tile's keys
+    // decides, the two halves meet only then
+    auto rescale = [&](float mx) {
+        if (__builtin_expect(__all(mx - m_run <= kRescaleSlack), 1)) return;
+        float a, b;
+        half_wave_pair(mx, a, b);
+        const float m_new = max_nan(m_run, max_nan(a, b)), alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+        m_run = m_new;
+        l_run *= alpha;
+        acc_scale_n<0, 16 * HD::kBlocks>(alpha);
+    };
 
+    constexpr int NS = HD::kSteps * KB, NE = 16 * KB, NV = 2 * KB * HD::kBlocks, AHEAD = 4;
+    int lim = 0;
+    unsigned groups = kAllGroups;
+    int specials = 0;  // masked tiles held infinities or NaN in V
+    int masked = 0;  // (whole numbers in scalar registers: a branch on a lane mask would keep both sides' registers alive)
+    // Q is waited for HERE: left pending, the waits in front of its uses would drain the loop's transfers
+#pragma unroll
+    for (int ks = 0; ks < HD::kSteps; ++ks) asm volatile("" : "+v"(qf[ks]));
     wait_all_vmem();
     __syncthreads();
-    for (int t = 0; t < n_tiles; ++t) {
-        const unsigned groups = on_page & ((1u << CPT) - 1);
-        if (t + ST - 1 < n_tiles) send(t + ST - 1);  // into the stage of tile t - 1, which every wave has left
-        on_page >>= CPT;
-        const int u = u0 + t;
-        // the last key of this tile that the row sees; a wave whose rows see none of it passes it by
-        const int lim = u < it.prefix_tiles ? p.prefix_len - 1 - u * TK : own_limit - (u - it.prefix_tiles) * TK;
-        if (wave_valid && __any(lim >= 0)) {
-            const char* kb = ring + (t % ST) * kStage;
-            const char* vb = kb + kTile;
-            f32x16 s[KB];
+    if constexpr (D == 64)
+        acc_reserve32();
+    else if constexpr (D == 128)
+        acc_reserve64();
+    else
+        acc_reserve128();
+    static_for<HD::kBlocks>([&](auto ic) { acc_zero16<16 * decltype(ic)::value>(); });
+    if (wave_valid && n_tiles > 0) {
+        lim = limit_of(0);
+        groups = on_page & kAllGroups;
+        masked = needs_mask(lim, groups);
 #pragma unroll
-            for (int b = 0; b < KB; ++b) {
+        for (int b = 0; b < KB; ++b)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) s[b][e] = 0.0f;
+            for (int e = 0; e < 16; ++e) s_cur[b][e] = 0.0f;
 #pragma unroll
-                for (int ks = 0; ks < HD::kSteps; ++ks)
-                    s[b] = Elem<E>::mfma(*reinterpret_cast<const v8*>(kb + geo.k_rd[ks] + b * 32 * HD::kRow), qf[ks], s[b]);
-            }
-            const bool masked = __any(lim < TK - 1) || groups != (1u << CPT) - 1;
-            if (masked) {
+        for (int i = 0; i < NS; ++i) s_cur[i % KB] = Elem<E>::mfma(k_frag(ring, i), qf[i / KB], s_cur[i % KB]);
+        if (masked) mask_scores(s_cur, lim, groups);
+        rescale(lane_max(s_cur));
+    }
+    // Step t: while the matrix pipe computes the next tile's scores, the vector ALU turns this tile's into probabilities; while
+    // it multiplies those with V, the vector ALU takes the next scores' maximum.  Written out gap by gap: one MFMA, that
+    // gap's share of the vector work, the operand read AHEAD MFMAs later, one piece of the step's transfer.
+    auto step = [&](int t, auto sends) {
+        constexpr bool kSend = decltype(sends)::value;  // tile t + ST - 1, into the stage of tile t - 1, which every wave has left
+        const bool more = kSend || t + 1 < n_tiles;
+        Transfer tr;
+        if constexpr (kSend) tr = transfer(t + ST - 1);
+        if (wave_valid) {
+            const char* kb = ring + ((t + 1) % ST) * kStage;
+            const char* vb = ring + (t % ST) * kStage + kTile;
+            v8 pf[2 * KB], kf[AHEAD], vf[AHEAD];
+            float sum = 0.0f;
 #pragma unroll
-                for (int b = 0; b < KB; ++b)
+            for (int b = 0; b < KB; ++b)
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const int k = 32 * b + 8 * (e >> 2) + (e & 3);
-                        if (k + 4 * geo.hh > lim || !((groups >> (k >> 4)) & 1)) s[b][e] = -__builtin_inff();
+                for (int e = 0; e < 16; ++e) s_next[b][e] = 0.0f;
+            // (past the last tile the scores of whatever the stage holds: never used)
+            static_for<AHEAD>([&](auto ic) { kf[decltype(ic)::value] = k_frag(kb, decltype(ic)::value); });
+            static_for<NS>([&](auto ic) {
+                constexpr int i = decltype(ic)::value;
+                s_next[i % KB] = Elem<E>::mfma(kf[i % AHEAD], qf[i / KB], s_next[i % KB]);
+                if constexpr (i + AHEAD < NS) kf[i % AHEAD] = k_frag(kb, i + AHEAD);
+                constexpr int every = NS / (2 * PPW);
+                if constexpr (kSend && i % every == every - 1) send_piece(tr, std::integral_constant<int, i / every>{});
+                static_for<NE / NS>([&](auto jc) {
+                    constexpr int e = i * (NE / NS) + decltype(jc)::value;
+                    const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s_cur[e / 16][e % 16], c, -m_run));
+                    s_cur[e / 16][e % 16] = x;
+                    if constexpr (e > 0) sum += s_cur[(e - 1) / 16][(e - 1) % 16];
+                    if constexpr (e % 2 == 1 && e >= 3) {
+                        pf[(e - 3) / 8][(e - 3) % 8] = (E)s_cur[(e - 3) / 16][(e - 3) % 16];
+                        pf[(e - 2) / 8][(e - 2) % 8] = (E)s_cur[(e - 2) / 16][(e - 2) % 16];
                     }
-            }
-            float mx = s[0][0];
+                });
+                __builtin_amdgcn_sched_barrier(0);
+            });
+            sum += s_cur[KB - 1][15];
+            l_run += sum;
+            pf[2 * KB - 1][6] = (E)s_cur[KB - 1][14];
+            pf[2 * KB - 1][7] = (E)s_cur[KB - 1][15];
+            // (pinned here: left alone the compiler sinks the vector work into the block that uses it)
 #pragma unroll
-            for (int b = 0; b < KB; ++b)
-#pragma unroll
-                for (int e = b == 0 ? 1 : 0; e < 16; ++e) mx = max_nan(mx, s[b][e]);
-            {
-                float a, b;
-                half_wave_pair(mx, a, b);
-                mx = max_nan(a, b) * p.scale_log2e;
-            }
-            if (!__all(mx - m_run <= kRescaleSlack)) {
-                const float m_new = max_nan(m_run, mx), alpha = __builtin_amdgcn_exp2f(m_run - m_new);
-                m_run = m_new;
-                l_run *= alpha;
-#pragma unroll
-                for (int db = 0; db < HD::kBlocks; ++db)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) oacc[db][e] *= alpha;
-            }
-            v8 pf[2 * KB];
-#pragma unroll
-            for (int b = 0; b < KB; ++b)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][e], p.scale_log2e, -m_run));
-                    l_run += x;
-                    pf[2 * b + e / 8][e % 8] = (E)x;
-                }
-            if (!masked) {
-#pragma unroll
-                for (int kk = 0; kk < 2 * KB; ++kk)
-#pragma unroll
-                    for (int db = 0; db < HD::kBlocks; ++db) oacc[db] = Elem<E>::mfma(v_frag(vb, kk, db), pf[kk], oacc[db]);
+            for (int j = 0; j < 2 * KB; ++j) asm volatile("" : "+v"(pf[j]));
+            asm volatile("s_nop 4" : "+v"(l_run));  // (wait states between a vector write and the MFMAs that read it)
+
+            const int lim_next = limit_of(t + 1);
+            const unsigned groups_next = (on_page >> CPT) & kAllGroups;
+            const int masked_next = needs_mask(lim_next, groups_next);
+            if (__builtin_expect(masked_next != 0, 0)) mask_scores(s_next, lim_next, groups_next);
+            float mx;
+            if (__builtin_expect(masked == 0, 1)) {
+                static_for<AHEAD>([&](auto ic) { vf[decltype(ic)::value] = v_frag(vb, decltype(ic)::value / HD::kBlocks, decltype(ic)::value % HD::kBlocks); });
+                mx = max_nan(s_next[0][0], s_next[0][1]);
+                static_for<NV>([&](auto ic) {
+                    constexpr int i = decltype(ic)::value;
+                    Elem<E>::template mfma_owned<16 * (i % HD::kBlocks)>(vf[i % AHEAD], pf[i / HD::kBlocks]);
+                    if constexpr (i + AHEAD < NV) vf[i % AHEAD] = v_frag(vb, (i + AHEAD) / HD::kBlocks, (i + AHEAD) % HD::kBlocks);
+                    if constexpr (i >= 2) {  // links of the maximum, from the third gap on
+                        constexpr int NL = 8 * KB - 1, lo = (i - 2) * NL / (NV - 2), hi = (i - 1) * NL / (NV - 2);
+                        static_for<hi - lo>([&](auto jc) {
+                            constexpr int e = 2 * (lo + decltype(jc)::value + 1);
+                            mx = max_nan(max_nan(mx, s_next[e / 16][e % 16]), s_next[e / 16][e % 16 + 1]);
+                        });
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                });
+                mx *= c;
             } else {
                 bool special = false;
-#pragma unroll
-                for (int kk = 0; kk < 2 * KB; ++kk)
-#pragma unroll
-                    for (int db = 0; db < HD::kBlocks; ++db)
-                        oacc[db] = Elem<E>::mfma(finite_part<E>(v_frag(vb, kk, db), special), pf[kk], oacc[db]);
-                if (__any(special)) {
-                    v8 sees[2 * KB];  // 1 where the row sees the key
-#pragma unroll
-                    for (int kk = 0; kk < 2 * KB; ++kk)
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const int k = 16 * kk + 8 * (i >> 2) + (i & 3);
-                            sees[kk][i] = (E)(k + 4 * geo.hh <= lim && ((groups >> (k >> 4)) & 1) ? 1.0f : 0.0f);
-                        }
-#pragma unroll 1
-                    for (int kind = 1; kind <= 3; ++kind) {
-#pragma unroll
-                        for (int db = 0; db < HD::kBlocks; ++db) {
-                            f32x16 n;
-#pragma unroll
-                            for (int e = 0; e < 16; ++e) n[e] = 0.0f;
-#pragma unroll
-                            for (int kk = 0; kk < 2 * KB; ++kk)
-                                n = Elem<E>::mfma(special_part<E>(v_frag(vb, kk, db), kind), sees[kk], n);
-#pragma unroll
-                            for (int e = 0; e < 16; ++e)
-                                if (n[e] > 0.0f) oacc[db][e] += special_value(kind);
-                        }
-                    }
-                }
+                static_for<NV>([&](auto ic) {
+                    constexpr int kk = decltype(ic)::value / HD::kBlocks, db = decltype(ic)::value % HD::kBlocks;
+                    v8 f = finite_part<E>(v_frag(vb, kk, db), special);
+                    asm volatile("s_nop 4" : "+v"(f));
+                    Elem<E>::template mfma_owned<16 * db>(f, pf[kk]);
+                });
+                specials |= __builtin_amdgcn_readfirstlane((int)__any(special));
+                mx = lane_max(s_next);
             }
+            if (more) {
+                rescale(mx);
+                lim = lim_next, groups = groups_next, masked = masked_next;
+#pragma unroll
+                for (int b = 0; b < KB; ++b) s_cur[b] = s_next[b];
+            }
+        } else if constexpr (kSend) {
+            static_for<2 * PPW>([&](auto ic) { send_piece(tr, ic); });
         }
-        // this wave's share of tile t + 1 has landed (transfers complete in order); the next ST - 2 stay in flight
-        if (t + ST - 1 < n_tiles)
-            asm volatile("s_waitcnt vmcnt(%0)" : : "n"((ST - 2) * 2 * PPW) : "memory");
+        on_page >>= CPT;
+        // this wave's share of tile t + 2 has landed (transfers complete in order); what was sent since stays in flight
+        if constexpr (kSend)
+            asm volatile("s_waitcnt vmcnt(%0)" : : "n"((ST - 3) * 2 * PPW) : "memory");
         else
             wait_all_vmem();
         __syncthreads();
+    };
+    int t = 0;
+    for (; t + ST - 1 < n_tiles; ++t) step(t, std::true_type{});
+    for (; t < n_tiles; ++t) step(t, std::false_type{});
+
+    acc_fence();
+    if (__builtin_expect(specials != 0, 0)) {
+        // the values taken out of masked tiles, to the rows that do see them: those tiles' V once more, in the quarter of the
+        // ring that is this wave's own now
+        char* mine = ring + wave * (ST * kStage / 4);
+        const unsigned mine_lds = ring_lds + (unsigned)(wave * (ST * kStage / 4));
+#pragma unroll 1
+        for (int t = 0; t < n_tiles; ++t) {
+            const int u = u0 + t, key = (u < it.prefix_tiles ? u : u - it.prefix_tiles) * TK, lim = limit_of(t);
+            unsigned groups = 0;
+#pragma unroll 1
+            for (int j = 0; j < kTile / 1024; ++j) {
+                const int row = RPP * j, page = __builtin_amdgcn_readfirstlane(page_of_group<TK>(p, it, t * CPT + row / 16, n_tiles * CPT));
+                groups |= page >= 0 ? 1u << (row / 16) : 0u;
+                const char* vb = v_head + 2 * ((int64_t)max(page, 0) * p.vs.page + (int64_t)((key + row) & P1) * p.vs.row);
+                dma16(mine_lds + 1024u * j, vb, (unsigned)(d_rip * (int)p.vs.row * 2) + (unsigned)((d_slot ^ (((row + d_rip) & HD::kVMask) << 2)) << 4));
+            }
+            wait_all_vmem();
+            if (!needs_mask(lim, groups)) continue;
+            v8 sees[2 * KB];  // 1 where the row sees the key
+#pragma unroll
+            for (int kk = 0; kk < 2 * KB; ++kk)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int k = 16 * kk + 8 * (i >> 2) + (i & 3);
+                    sees[kk][i] = (E)(k + 4 * geo.hh <= lim && ((groups >> (k >> 4)) & 1) ? 1.0f : 0.0f);
+                }
+            static_for<HD::kBlocks>([&](auto dc) {
+                constexpr int db = decltype(dc)::value;
+#pragma unroll 1
+                for (int kind = 1; kind <= 3; ++kind) {
+                    f32x16 n;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) n[e] = 0.0f;
+#pragma unroll
+                    for (int kk = 0; kk < 2 * KB; ++kk) n = Elem<E>::mfma(special_part<E>(v_frag(mine, kk, db), kind), sees[kk], n);
+                    static_for<16>([&](auto ec) {
+                        constexpr int e = decltype(ec)::value;
+                        const float x = acc_get<16 * db + e>();
+                        acc_put<16 * db + e>(n[e] > 0.0f ? x + special_value(kind) : x);
+                    });
+                }
+            });
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        }
     }
 
     if (!valid) return;
@@ -721,34 +871,29 @@ __device__ __forceinline__ void shared_many_rows(const SharedPrefixParams& p, co
     if (!it.stacked && it.part == 0 && geo.hh == 0) p.row_parts[row] = total == 1 ? 0 : total;
     if (!it.stacked && total == 1) {
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        uint16_t* og = p.o + tok * p.o_tok + hq * p.o_head;
-#pragma unroll
-        for (int db = 0; db < HD::kBlocks; ++db)
-#pragma unroll
-            for (int g4 = 0; g4 < 4; ++g4) {
-                typename Elem<E>::v4 x;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] = (E)(oacc[db][4 * g4 + e] * inv);
-                *reinterpret_cast<typename Elem<E>::v4*>(og + 32 * db + 8 * g4 + 4 * geo.hh) = x;
-            }
+        uint16_t* og = p.o + tok * p.o_tok + hq * p.o_head + 4 * geo.hh;
+        static_for<HD::kBlocks * 4>([&](auto ic) {
+            constexpr int i = decltype(ic)::value;
+            const typename Elem<E>::v4 x = {(E)(acc_get<4 * i>() * inv), (E)(acc_get<4 * i + 1>() * inv), (E)(acc_get<4 * i + 2>() * inv),
+                                            (E)(acc_get<4 * i + 3>() * inv)};
+            *reinterpret_cast<typename Elem<E>::v4*>(og + 8 * i) = x;
+        });
         return;
     }
     const int64_t slot = part_slot(p, it, row);
     if (geo.hh == 0) *reinterpret_cast<f32x2*>(p.part_ml + 2 * slot) = f32x2{m_run, l};
     if (n_tiles == 0) return;  // (nothing is read of a part whose sum is 0)
-    float* oa = p.part_o + slot * D;
-#pragma unroll
-    for (int db = 0; db < HD::kBlocks; ++db)
-#pragma unroll
-        for (int g4 = 0; g4 < 4; ++g4) {
-            const f32x4 x = {oacc[db][4 * g4], oacc[db][4 * g4 + 1], oacc[db][4 * g4 + 2], oacc[db][4 * g4 + 3]};
-            *reinterpret_cast<f32x4*>(oa + 32 * db + 8 * g4 + 4 * geo.hh) = x;
-        }
+    float* oa = p.part_o + slot * D + 4 * geo.hh;
+    static_for<HD::kBlocks * 4>([&](auto ic) {
+        constexpr int i = decltype(ic)::value;
+        *reinterpret_cast<f32x4*>(oa + 8 * i) = f32x4{acc_get<4 * i>(), acc_get<4 * i + 1>(), acc_get<4 * i + 2>(), acc_get<4 * i + 3>()};
+    });
 }
 
 template <typename E, int D>
-__global__ __launch_bounds__(256, SharedCfg<D>::kOcc) void fa_shared_prefix_kernel(const SharedPrefixParams p) {
-    constexpr int TK = SharedCfg<D>::kTk;
+__device__ __forceinline__ void shared_prefix_body(const SharedPrefixParams& p) {
+    using CFG = SharedCfg<D>;
+    constexpr int TK = CFG::kTk;
     __shared__ __attribute__((aligned(1024))) char ring[SharedCfg<D>::kStages * 2 * TK * 2 * D];
     SharedItem it;
     int toks[2];  // of this lane's rows: 32 wave + (lane & 31), or, of few rows, (lane & 15) and 16 + (lane & 15)
@@ -784,7 +929,7 @@ __global__ __launch_bounds__(256, SharedCfg<D>::kOcc) void fa_shared_prefix_kern
         it.before = first > 0 ? plan.prefix_parts : 0;  // (parts that P items add in front of this item's)
         it.u0 = first + (int)((int64_t)(last - first) * it.part / it.parts);
         it.n_tiles = first + (int)((int64_t)(last - first) * (it.part + 1) / it.parts) - it.u0;
-        few = end - it.row0 <= 32;
+        few = end - it.row0 <= 16 * CFG::kFewBlocks;
         auto token = [&](int off) -> int {
             const int t = min(it.row0 + off, it.rows - 1) / p.g;
             if (!it.stacked) return tok0 + t;
@@ -797,11 +942,23 @@ __global__ __launch_bounds__(256, SharedCfg<D>::kOcc) void fa_shared_prefix_kern
     }
     if (!few)
         shared_many_rows<E, D>(p, it, toks[0], ring);
-    else if (min(it.rows - it.row0, kRowTile) <= 16)
+    else if (CFG::kFewBlocks == 1 || min(it.rows - it.row0, kRowTile) <= 16)
         shared_few_rows<E, D, 1>(p, it, toks, ring);
     else
-        shared_few_rows<E, D, 2>(p, it, toks, ring);
+        shared_few_rows<E, D, CFG::kFewBlocks>(p, it, toks, ring);
 }
+
+// Two workgroups share a compute unit (D = 64, 128): architectural and accumulator registers together within 256.  The
+// compiler halves that between the two kinds when asked for two; it is asked for one, with the architectural count given.
+#define FA_SHARED_KERNEL(name, E, D, VGPRS) \
+    __global__ __launch_bounds__(256, 1) __attribute__((amdgpu_num_vgpr(VGPRS))) void name(const SharedPrefixParams p) { shared_prefix_body<E, D>(p); }
+FA_SHARED_KERNEL(fa_shared_prefix_f16_d64_kernel, _Float16, 64, 224)
+FA_SHARED_KERNEL(fa_shared_prefix_f16_d128_kernel, _Float16, 128, 192)
+FA_SHARED_KERNEL(fa_shared_prefix_f16_d256_kernel, _Float16, 256, 256)
+FA_SHARED_KERNEL(fa_shared_prefix_bf16_d64_kernel, __bf16, 64, 224)
+FA_SHARED_KERNEL(fa_shared_prefix_bf16_d128_kernel, __bf16, 128, 192)
+FA_SHARED_KERNEL(fa_shared_prefix_bf16_d256_kernel, __bf16, 256, 256)
+#undef FA_SHARED_KERNEL
 
 // O = sum_s w_s o_s / sum_s w_s l_s,  w_s = exp2(m_s - max_s m_s): D / 4 lanes per row, four parts in flight.  Rows of no
 // request and rows that are written already are left alone.

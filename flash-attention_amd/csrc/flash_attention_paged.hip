@@ -111,8 +111,12 @@ int check_shared(int T, int B, int Hq, int Hkv, int prefix_len, int max_k_len) {
 template <typename E, int D>
 int launch_shared(const fa::SharedPrefixParams& p, const Bounds& d, hipStream_t stream) {
     if (d.blocks > 0x7fffffffLL) return fail(FA_ERR_SHAPE, "fa_forward_shared_prefix: grid size out of range");
-    hipLaunchKernelGGL((fa::fa_shared_prefix_kernel<E, D>), dim3((unsigned)d.blocks), dim3(256), 0, stream, p);
-    if (int rc = hip_ok(hipGetLastError(), "fa_shared_prefix_kernel")) return rc;
+    constexpr bool half = std::is_same<E, _Float16>::value;
+    void (*const kernel)(fa::SharedPrefixParams) = D == 64    ? (half ? fa::fa_shared_prefix_f16_d64_kernel : fa::fa_shared_prefix_bf16_d64_kernel)
+                                                   : D == 128 ? (half ? fa::fa_shared_prefix_f16_d128_kernel : fa::fa_shared_prefix_bf16_d128_kernel)
+                                                              : (half ? fa::fa_shared_prefix_f16_d256_kernel : fa::fa_shared_prefix_bf16_d256_kernel);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)d.blocks), dim3(256), 0, stream, p);
+    if (int rc = hip_ok(hipGetLastError(), "fa_shared_prefix kernel")) return rc;
     constexpr int rows = 256 / (D / 4);
     const int64_t merge = ((int64_t)p.T * p.Hkv * p.g + rows - 1) / rows;
     hipLaunchKernelGGL((fa::fa_shared_prefix_merge_kernel<E, D>), dim3((unsigned)merge), dim3(256), 0, stream, p);

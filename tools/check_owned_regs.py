@@ -1,6 +1,6 @@
 #!/usr/bin/env python3
 """Build-time audit of the kernels whose inline asm owns accumulator registers: fa_fwd_w64_kernel, its masked
-forms (causal, ragged, both) and its key-split form, and the fa_fwd_hd_kernel family.
+forms (causal, ragged, both) and its key-split form, the fa_fwd_hd_kernel family and the fa_shared_prefix kernels.
 
 These kernels name a[..] literally in their instruction strings; the compiler does not know they hold
 live values.  That is only sound while the compiler itself uses no accumulator register and spills
@@ -31,6 +31,12 @@ KERNELS = ["_ZN2fa17fa_fwd_w64_kernelENS_9FwdParamsE", "_ZN2fa24fa_fwd_w64_causa
            "_ZN2fa22fa_fwd_hd_state_kernelILi64EEEvNS_9FwdParamsE", "_ZN2fa22fa_fwd_hd_state_kernelILi128EEEvNS_9FwdParamsE",
            "_ZN2fa22fa_fwd_hd_state_kernelILi256EEEvNS_9FwdParamsE"]
 
+# the shared-prefix kernels: another translation unit, with its own flags (csrc/Makefile's PAGEDFLAGS)
+PAGED_SRC = os.path.join(ROOT, "flash-attention_amd", "csrc", "flash_attention_paged.hip")
+PAGED_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-mllvm", "-amdgpu-mfma-vgpr-form=1"]
+PAGED_KERNELS = ["_ZN2fa%dfa_shared_prefix_%s_d%d_kernelENS_18SharedPrefixParamsE" % (len("fa_shared_prefix_%s_d%d_kernel" % (e, d)), e, d)
+                 for e in ("f16", "bf16") for d in (64, 128, 256)]
+
 
 def main():
     src = os.environ.get("FA_AUDIT_SRC", SRC)
@@ -45,6 +51,14 @@ def main():
             open(os.environ["FA_AUDIT_KEEP"], "w").write(text)
     for kernel in kernels:
         audit(text, kernel)
+    if not os.environ.get("FA_AUDIT_KERNELS") and not sys.argv[1:]:
+        with tempfile.TemporaryDirectory() as tmp:
+            out = os.path.join(tmp, "paged.s")
+            subprocess.run(["/opt/rocm/bin/hipcc", "-O3", "-std=c++17", "--offload-arch=gfx950"] + PAGED_FLAGS +
+                           ["-S", "--cuda-device-only", "-o", out, PAGED_SRC], check=True, stderr=subprocess.DEVNULL)
+            text = open(out).read()
+        for kernel in PAGED_KERNELS:
+            audit(text, kernel)
     print("check_owned_regs: ok (no spills, no scratch, no compiler use of accumulator registers)")
 
 
