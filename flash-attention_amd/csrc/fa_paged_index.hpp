@@ -40,8 +40,8 @@ FA_HD int slot_of(int page, int row, int log2_page) {
 // How a launch of shared-prefix attention is divided.  Row tiles of 128 rows walk `tiles` key tiles each, in `parts_for`
 // ranges of about `steps_for` key tiles: all key tiles of the launch (`work`, per K/V head) over the workgroups that the
 // chip holds (`slots`).  With x = tiles / steps a row tile has max(1, floor(x + 1/2)) ranges at most, i.e. fewer than x
-// beyond the first, and all x together are at most `slots`: blocks_bound holds for any lengths (with half as much again for
-// the rounding of the sum).
+// beyond the first, and all x together are at most `slots`; the stacked rows' ranges may be made as many as `slots` besides.
+// So blocks_bound holds for any lengths (with half of `slots` for the rounding of the sum).
 constexpr int kRowTile = 128;
 FA_HD int row_tiles(int64_t rows) { return (int)((rows + kRowTile - 1) / kRowTile); }
 FA_HD int parts_for(int tiles, int steps, int most) {
@@ -57,8 +57,21 @@ FA_HD int steps_for(float work, int heads, int slots, int least) {
 // Row tiles of a batch of `requests` with `rows` rows in all, and its workgroups.
 FA_HD int64_t request_tiles_bound(int64_t rows, int requests) { return rows / kRowTile + requests; }
 FA_HD int64_t blocks_bound(int64_t prefix_row_tiles, int64_t request_row_tiles, int heads, int slots) {
-    return heads * (prefix_row_tiles + request_row_tiles) + 3 * (int64_t)slots / 2 + 1;
+    return heads * (prefix_row_tiles + request_row_tiles) + 5 * (int64_t)slots / 2 + 1;
 }
+
+// a / b for 0 <= a < 2^31, 1 <= b, from a reciprocal r of b that is good to 1 ulp (v_rcp_f32): the first quotient is off by
+// 2^-22 of itself and one at most, the second by one.
+FA_HD int div_by(int a, int b, float r) {
+    const float f = (float)a * r;
+    int q = f >= 2147483520.0f ? 2147483520 : (int)f;
+    unsigned m = (unsigned)a - (unsigned)q * (unsigned)b;
+    q += (int)((float)(int)m * r);
+    const int e = (int)((unsigned)a - (unsigned)q * (unsigned)b);
+    return e < 0 ? q - 1 : e >= b ? q + 1 : q;
+}
+// 2^32 / g rounded up: R / g is the high word of R times this for R g < 2^32 (g = 1 apart, which needs none).
+FA_HD unsigned group_reciprocal(int g) { return (unsigned)((((uint64_t)1 << 32) + g - 1) / g); }
 
 // One request's step, from its lengths alone.  keys held (clamped to what a table row names), keys after the step,
 // pages before and after; `wide`: the step asks for more than the row of the table can name.

@@ -39,9 +39,12 @@ struct SharedPrefixParams {
     int* row_parts;   // [T * Hq]: parts of the row's sum; 0: its output is written already
     int T, B, Hkv, g, log2_page, n_pages, prefix_len, table_width, causal;
     float scale_log2e;
-    int slots;                      // workgroups that the chip holds at a time
+    int slots, two_per_unit;        // workgroups that the chip holds at a time; whether two share a compute unit
+    int few_rows;                   // up to this many rows take the form for few
+    unsigned g_reciprocal;          // 2^32 / g, rounded up
     int max_prefix_parts, max_own_parts;
 };
+constexpr int kManyCost = 2;
 
 template <typename E>
 struct Elem;
@@ -126,101 +129,130 @@ struct SharedCfg<256> {
     static constexpr int kTk = 32, kStages = 4, kFewBlocks = 1;  // 32 KiB
 };
 
-// The division of a launch into workgroups, from the requests' lengths; every workgroup computes it for itself.
+// The division of a launch into workgroups, from the requests' lengths; every wave computes it for itself (no barrier: all
+// write the same numbers to LDS, each reads what it has written).
 //   A request with fewer than 128 rows (new tokens x g) is short: its rows are stacked up with those of the other short
 // requests against the prefix (items of kind P: one K/V head, 128 stacked rows, a range of the prefix) and alone against
 // its own keys (O: one head, the request's rows, a range of its keys).  A longer request fills row tiles of its own, which walk
 // prefix and own keys in one go (J: one head, 128 of its rows, a range of both): nothing is gained by stacking.
-//   Ranges are `steps` key tiles long, up to half a range more or less: all tiles of the launch over the workgroups that
-// the chip holds.
+//   Ranges take about the same time each, up to half more or less: the launch's key tiles over the workgroups that the chip
+// holds, a tile of many rows counted as kManyCost tiles of few.
 struct SharedPlan {
     int stacked;        // rows of the short requests, per K/V head
     int prefix_tiles;   // key tiles of the prefix
     int prefix_parts;   // ranges of the prefix that P items walk
     int p_items;
-    int steps;
+    int steps_few, steps_many;  // key tiles of a range
 };
-
-// Inclusive sum over the 256 threads of a workgroup; `total` for everybody.  `tmp`: 4 ints of LDS.
-__device__ __forceinline__ int workgroup_sum(int v, int* tmp, int& total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int u = __shfl_up(v, d);
-        if (lane >= d) v += u;
+// LDS, until the first transfer: per request its first token, its own keys, the stacked tokens and the items before it.
+struct SharedTables {
+    int *tok0, *keys, *stacked, *items;
+    __device__ __forceinline__ SharedTables(char* lds, int B) {
+        tok0 = reinterpret_cast<int*>(lds);
+        keys = tok0 + B + 1;
+        stacked = keys + B;
+        items = stacked + B;
     }
-    __syncthreads();
-    if (lane == 63) tmp[wave] = v;
-    __syncthreads();
-    const int a = tmp[0], b = tmp[1], c = tmp[2];
-    total = a + b + c + tmp[3];
-    return v + (wave > 0 ? a : 0) + (wave > 1 ? b : 0) + (wave > 2 ? c : 0);
-}
-
-struct SharedRequest {
-    int tok0, n, keys;
 };
-__device__ __forceinline__ SharedRequest shared_request(const SharedPrefixParams& p, int b) {
-    SharedRequest r;
-    r.tok0 = clamp_int(p.q_start[b], 0, p.T);
-    r.n = clamp_int(p.q_start[b + 1], r.tok0, p.T) - r.tok0;
-    r.keys = clamp_int(p.k_len[b], 0, p.table_width << p.log2_page);
-    return r;
+
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_int(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, true); }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float dpp_float(float v) { return __builtin_bit_cast(float, dpp_int<CTRL, ROWS>(__builtin_bit_cast(int, v))); }
+// Inclusive sum over the wave: within rows of 16 lanes, then row ends into the rows above.
+__device__ __forceinline__ int wave_sum_up(int v) {
+    v += dpp_int<0x111, 0xf>(v);
+    v += dpp_int<0x112, 0xf>(v);
+    v += dpp_int<0x114, 0xf>(v);
+    v += dpp_int<0x118, 0xf>(v);
+    v += dpp_int<0x142, 0xa>(v);
+    v += dpp_int<0x143, 0xc>(v);
+    return v;
+}
+__device__ __forceinline__ float wave_total(float v) {
+    v += dpp_float<0x111, 0xf>(v);
+    v += dpp_float<0x112, 0xf>(v);
+    v += dpp_float<0x114, 0xf>(v);
+    v += dpp_float<0x118, 0xf>(v);
+    v += dpp_float<0x142, 0xa>(v);
+    v += dpp_float<0x143, 0xc>(v);
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+}
+__device__ __forceinline__ int quick_div(int a, int b) { return div_by(a, b, __builtin_amdgcn_rcpf((float)b)); }
+// R / g for the rows of a launch (R g < 2^32: the launcher's check), by the reciprocal 2^32 / g rounded up.
+__device__ __forceinline__ int div_group(const SharedPrefixParams& p, int R) { return p.g == 1 ? R : (int)__umulhi((unsigned)R, p.g_reciprocal); }
+
+__device__ __forceinline__ int quick_parts(int tiles, int steps, int most) { return max(1, min(quick_div(tiles + (steps >> 1), steps), most)); }
+
+template <int TK>
+__device__ __forceinline__ int request_parts(const SharedPrefixParams& p, const SharedPlan& s, int rows, int keys) {
+    const int own = (keys + TK - 1) / TK;
+    return rows >= kRowTile ? quick_parts(s.prefix_tiles + own, s.steps_many, p.max_prefix_parts + p.max_own_parts)
+                            : quick_parts(own, rows <= p.few_rows ? s.steps_few : s.steps_many, p.max_own_parts);
 }
 
-// Items of a request; 0 where it has no rows.
+// Returns the number of items.
 template <int TK>
-__device__ __forceinline__ int request_items(const SharedPrefixParams& p, const SharedPlan& s, const SharedRequest& r, int& tiles, int& parts) {
-    const int rows = r.n * p.g, own = (r.keys + TK - 1) / TK;
-    tiles = (rows + 127) >> 7;
-    parts = rows >= 128 ? parts_for(s.prefix_tiles + own, s.steps, p.max_prefix_parts + p.max_own_parts) : parts_for(own, s.steps, p.max_own_parts);
-    return tiles * parts * p.Hkv;
-}
-
-// LDS: stacked_start[B] (stacked tokens before request b), item_start[B] (items before it, P items among them).
-template <int TK>
-__device__ __forceinline__ int shared_plan(const SharedPrefixParams& p, SharedPlan& s, int* stacked_start, int* item_start, int* tmp) {
+__device__ __forceinline__ int shared_plan(const SharedPrefixParams& p, SharedPlan& s, const SharedTables& tab) {
+    const int lane = threadIdx.x & 63;
     s.prefix_tiles = (p.prefix_len + TK - 1) / TK;
     int tokens = 0;
-    float work = 0.0f;  // key tiles of all row tiles, per K/V head
+    float few = 0.0f, many = 0.0f;  // key tiles of all row tiles, per K/V head
     for (int b0 = 0; b0 < p.B; b0 += 256) {
-        const int b = b0 + (int)threadIdx.x;
-        int n = 0;
-        if (b < p.B) {
-            const SharedRequest r = shared_request(p, b);
-            const int rows = r.n * p.g, own = (r.keys + TK - 1) / TK;
-            if (rows < 128) n = r.n;
-            work += (float)((rows + 127) >> 7) * (float)(own + (rows < 128 ? 0 : s.prefix_tiles));
-        }
-        int total;
-        const int sum = workgroup_sum(n, tmp, total);
-        if (b < p.B) stacked_start[b] = tokens + sum - n;
-        tokens += total;
-    }
+        int q0[4], q1[4], k[4];
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) work += __shfl_xor(work, d);
-    float* ftmp = reinterpret_cast<float*>(tmp);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) ftmp[threadIdx.x >> 6] = work;
-    __syncthreads();
-    work = ftmp[0] + ftmp[1] + ftmp[2] + ftmp[3];
+        for (int i = 0; i < 4; ++i) {
+            const int b = min(b0 + 64 * i + lane, p.B - 1);
+            q0[i] = p.q_start[b], q1[i] = p.q_start[b + 1], k[i] = p.k_len[b];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (b0 + 64 * i >= p.B) break;
+            const int b = b0 + 64 * i + lane;
+            const int tok0 = clamp_int(q0[i], 0, p.T), keys = clamp_int(k[i], 0, p.table_width << p.log2_page);
+            const int n = b < p.B ? clamp_int(q1[i], tok0, p.T) - tok0 : 0, rows = n * p.g, own = (keys + TK - 1) / TK;
+            const int stacked = rows < kRowTile ? n : 0, sum = wave_sum_up(stacked);
+            if (b < p.B) {
+                tab.tok0[b] = tok0;
+                tab.keys[b] = keys;
+                tab.stacked[b] = tokens + sum - stacked;
+                if (b == p.B - 1) tab.tok0[p.B] = tok0 + n;
+                if (rows >= kRowTile)
+                    many += (float)row_tiles(rows) * (float)(own + s.prefix_tiles);
+                else if (rows > p.few_rows)
+                    many += (float)own;
+                else if (rows > 0)
+                    few += (float)own;
+            }
+            tokens += __builtin_amdgcn_readlane(sum, 63);
+        }
+    }
     s.stacked = tokens * p.g;
-    const int p_tiles = (s.stacked + 127) >> 7;
-    work += (float)p_tiles * (float)s.prefix_tiles;
-    s.steps = steps_for(work, p.Hkv, p.slots, 128 / TK);
-    s.prefix_parts = s.prefix_tiles > 0 && p_tiles > 0 ? parts_for(s.prefix_tiles, s.steps, p.max_prefix_parts) : 0;
+    const int p_tiles = row_tiles(s.stacked);
+    const bool p_few = s.stacked <= p.few_rows;
+    few = wave_total(few), many = wave_total(many);
+    const float prefix = (float)p_tiles * (float)s.prefix_tiles;
+    (p_few ? few : many) += prefix;
+    s.steps_few = steps_for(few + (float)kManyCost * many, p.Hkv, p.slots, 128 / TK);
+    s.steps_many = max(128 / TK, (s.steps_few + kManyCost - 1) / kManyCost);
+    s.prefix_parts = 0;
+    if (s.prefix_tiles > 0 && p_tiles > 0) {
+        s.prefix_parts = quick_parts(s.prefix_tiles, p_few ? s.steps_few : s.steps_many, p.max_prefix_parts);
+        // Two workgroups to a unit: more than one P item a unit but fewer than two leaves units with two, which take twice as
+        // long.  One on each, beside the launch's other items, or two on each where there is little else.
+        const int units = p_tiles * p.Hkv, half = p.slots >> 1;
+        if (p.two_per_unit && units * s.prefix_parts > half && units * s.prefix_parts < p.slots)
+            s.prefix_parts = max(1, min(quick_div(prefix * 4.0f >= 3.0f * (few * (1.0f / kManyCost) + many) ? p.slots : half, units), p.max_prefix_parts));
+    }
     s.p_items = p_tiles * s.prefix_parts * p.Hkv;
     int items = s.p_items;
-    for (int b0 = 0; b0 < p.B; b0 += 256) {
-        const int b = b0 + (int)threadIdx.x;
-        int n = 0, tiles, parts;
-        if (b < p.B) n = request_items<TK>(p, s, shared_request(p, b), tiles, parts);
-        int total;
-        const int sum = workgroup_sum(n, tmp, total);
-        if (b < p.B) item_start[b] = items + sum - n;
-        items += total;
+    for (int b0 = 0; b0 < p.B; b0 += 64) {
+        const int b = b0 + lane, i = min(b, p.B - 1);
+        const int rows = max(tab.tok0[i + 1] - tab.tok0[i], 0) * p.g;
+        const int n = b < p.B ? row_tiles(rows) * request_parts<TK>(p, s, rows, tab.keys[i]) * p.Hkv : 0, sum = wave_sum_up(n);
+        if (b < p.B) tab.items[b] = items + sum - n;
+        items += __builtin_amdgcn_readlane(sum, 63);
     }
-    __syncthreads();
     return items;
 }
 
@@ -228,8 +260,8 @@ __device__ __forceinline__ int shared_plan(const SharedPrefixParams& p, SharedPl
 // K/V head and a range) follow each other on one XCD (workgroup ids congruent mod 8 share one and its L2).
 __device__ __forceinline__ void unit_and_tile(int x, int units, int tiles, int& unit, int& tile) {
     const int full = units >> 3, per = 8 * tiles;
-    const int grp = min(x / per, full), r = x - grp * per, w = grp < full ? 8 : units & 7;
-    tile = r / w;
+    const int grp = min(quick_div(x, per), full), r = x - grp * per, w = grp < full ? 8 : units & 7;
+    tile = quick_div(r, w);
     unit = grp * 8 + (r - tile * w);
 }
 
@@ -301,7 +333,7 @@ __device__ __forceinline__ void shared_few_rows(const SharedPrefixParams& p, con
     v8 qf[RB][D / 32];
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
-        const int R = min(it.row0 + 16 * rb + r16, it.rows - 1), ti = R / p.g;
+        const int R = min(it.row0 + 16 * rb + r16, it.rows - 1), ti = div_group(p, R);
         hq[rb] = it.head * p.g + (R - ti * p.g);
         limit[rb] = p.causal ? min(it.own_keys - 1, it.own_keys - it.n_tok + ti) : it.own_keys - 1;
         const uint16_t* qr = p.q + toks[rb] * p.q_tok + hq[rb] * p.q_head + q4 * 8;
@@ -573,7 +605,7 @@ __device__ __forceinline__ void shared_many_rows(const SharedPrefixParams& p, co
     const int P1 = (1 << p.log2_page) - 1;  // (row in a page)
     const int R_off = wave * 32 + geo.r, head = it.head, row0 = it.row0, rows = it.rows, u0 = it.u0, n_tiles = it.n_tiles;
     const bool valid = row0 + R_off < rows, wave_valid = row0 + wave * 32 < rows;
-    const int R = min(row0 + R_off, rows - 1), ti = R / p.g, hq = head * p.g + (R - ti * p.g), Hq = p.Hkv * p.g;
+    const int R = min(row0 + R_off, rows - 1), ti = div_group(p, R), hq = head * p.g + (R - ti * p.g), Hq = p.Hkv * p.g;
     const int own_limit = p.causal ? min(it.own_keys - 1, it.own_keys - it.n_tok + ti) : it.own_keys - 1;  // the last own key this row sees
 
     // ---- transfers: this wave moves rows RPW * wave .. of each tile.  They lie on one page, whose number is uniform: lane L
@@ -862,32 +894,51 @@ __device__ __forceinline__ void shared_many_rows(const SharedPrefixParams& p, co
         }
     }
 
-    if (!valid) return;
-    const int64_t row = (int64_t)tok * Hq + hq;
+    // ---- out: whole rows, through the quarter of the ring that is this wave's own now (stored from the accumulator's layout a
+    //      wave instruction would touch 32 rows with 32 bytes each); chunk c of row r lies at c ^ (r & 15)
     float l0, l1;
     half_wave_pair(l_run, l0, l1);
     const float l = l0 + l1;
-    const int total = it.before + it.parts;
-    if (!it.stacked && it.part == 0 && geo.hh == 0) p.row_parts[row] = total == 1 ? 0 : total;
-    if (!it.stacked && total == 1) {
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        uint16_t* og = p.o + tok * p.o_tok + hq * p.o_head + 4 * geo.hh;
+    const int total = it.before + it.parts, row = tok * Hq + hq;
+    const bool direct = !it.stacked && total == 1;
+    if (valid && geo.hh == 0) {
+        if (!it.stacked && it.part == 0) p.row_parts[row] = direct ? 0 : total;
+        if (!direct) *reinterpret_cast<f32x2*>(p.part_ml + 2 * part_slot(p, it, row)) = f32x2{m_run, l};
+    }
+    if (!wave_valid || (n_tiles == 0 && !direct)) return;  // (nothing is read of a part whose sum is 0)
+    const float scale = !direct ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+    char* st = ring + wave * (ST * kStage / 4);
+    if (direct) {
+        constexpr int CH = D / 8;  // 16-byte chunks of an output row
         static_for<HD::kBlocks * 4>([&](auto ic) {
             constexpr int i = decltype(ic)::value;
-            const typename Elem<E>::v4 x = {(E)(acc_get<4 * i>() * inv), (E)(acc_get<4 * i + 1>() * inv), (E)(acc_get<4 * i + 2>() * inv),
-                                            (E)(acc_get<4 * i + 3>() * inv)};
-            *reinterpret_cast<typename Elem<E>::v4*>(og + 8 * i) = x;
+            const typename Elem<E>::v4 x = {(E)(acc_get<4 * i>() * scale), (E)(acc_get<4 * i + 1>() * scale), (E)(acc_get<4 * i + 2>() * scale),
+                                            (E)(acc_get<4 * i + 3>() * scale)};
+            *reinterpret_cast<u32x2*>(st + geo.r * 2 * D + ((i ^ (geo.r & (CH - 1) & 15)) << 4) + 8 * geo.hh) = __builtin_bit_cast(u32x2, x);
         });
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < CH / 2; ++i) {
+            const int r = i * (64 / CH) + lane / CH, c = lane % CH, tk = __shfl(tok, r), h = __shfl(hq, r);
+            const u32x4 x = *reinterpret_cast<const u32x4*>(st + r * 2 * D + ((c ^ (r & (CH - 1) & 15)) << 4));
+            if (row0 + wave * 32 + r < rows) *reinterpret_cast<u32x4*>(p.o + tk * p.o_tok + h * p.o_head + 8 * c) = x;
+        }
         return;
     }
-    const int64_t slot = part_slot(p, it, row);
-    if (geo.hh == 0) *reinterpret_cast<f32x2*>(p.part_ml + 2 * slot) = f32x2{m_run, l};
-    if (n_tiles == 0) return;  // (nothing is read of a part whose sum is 0)
-    float* oa = p.part_o + slot * D + 4 * geo.hh;
+    constexpr int CH = D / 4;  // 16-byte chunks of a row of the state
     static_for<HD::kBlocks * 4>([&](auto ic) {
         constexpr int i = decltype(ic)::value;
-        *reinterpret_cast<f32x4*>(oa + 8 * i) = f32x4{acc_get<4 * i>(), acc_get<4 * i + 1>(), acc_get<4 * i + 2>(), acc_get<4 * i + 3>()};
+        *reinterpret_cast<f32x4*>(st + geo.r * 4 * D + (((2 * i + geo.hh) ^ (geo.r & 15)) << 4)) =
+            f32x4{acc_get<4 * i>(), acc_get<4 * i + 1>(), acc_get<4 * i + 2>(), acc_get<4 * i + 3>()};
     });
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    float* po = p.part_o + part_slot(p, it, 0) * D;
+#pragma unroll 4
+    for (int i = 0; i < CH / 2; ++i) {
+        const int r = i * (64 / CH) + lane / CH, c = lane % CH, rw = __shfl(row, r);
+        const f32x4 x = *reinterpret_cast<const f32x4*>(st + r * 4 * D + ((c ^ (r & 15)) << 4));
+        if (row0 + wave * 32 + r < rows) *reinterpret_cast<f32x4*>(po + (int64_t)rw * D + 4 * c) = x;
+    }
 }
 
 template <typename E, int D>
@@ -899,45 +950,49 @@ __device__ __forceinline__ void shared_prefix_body(const SharedPrefixParams& p) 
     int toks[2];  // of this lane's rows: 32 wave + (lane & 31), or, of few rows, (lane & 15) and 16 + (lane & 15)
     bool few;
     {
-        int* stacked_start = reinterpret_cast<int*>(ring);  // (free until the first transfer)
-        int* item_start = stacked_start + p.B;
-        __shared__ int tmp[4];
+        const SharedTables tab(ring, p.B);  // (free until the first transfer)
         SharedPlan plan;
         const int x = (int)blockIdx.x, lane = threadIdx.x & 63;
-        if (x >= shared_plan<TK>(p, plan, stacked_start, item_start, tmp)) return;
+        if (x >= shared_plan<TK>(p, plan, tab)) return;
         it.prefix_tiles = plan.prefix_tiles;
         it.stacked = x < plan.p_items;
-        int unit, tile, tiles, b = 0, tok0 = 0;
+        int unit, tile, tiles, tok0 = 0, first_item = 0;
         it.own_keys = it.n_tok = 0;
         it.own_table = nullptr;
         if (it.stacked) {
             it.rows = plan.stacked, it.parts = plan.prefix_parts, tiles = row_tiles(plan.stacked);
         } else {
-            b = last_at_most(item_start, p.B, x);
-            const SharedRequest r = shared_request(p, b);
-            request_items<TK>(p, plan, r, tiles, it.parts);
-            it.rows = r.n * p.g, it.n_tok = r.n, it.own_keys = r.keys, tok0 = r.tok0;
+            const int b = last_at_most(tab.items, p.B, x);
+            tok0 = __builtin_amdgcn_readfirstlane(tab.tok0[b]);
+            it.n_tok = max(__builtin_amdgcn_readfirstlane(tab.tok0[b + 1]) - tok0, 0);
+            it.own_keys = __builtin_amdgcn_readfirstlane(tab.keys[b]);
+            first_item = __builtin_amdgcn_readfirstlane(tab.items[b]);
+            it.rows = it.n_tok * p.g;
+            tiles = row_tiles(it.rows);
+            it.parts = __builtin_amdgcn_readfirstlane(request_parts<TK>(p, plan, it.rows, it.own_keys));
             it.own_table = p.block_table + b * p.table_stride;
         }
-        unit_and_tile(x - (it.stacked ? 0 : item_start[b]), p.Hkv * it.parts, tiles, unit, tile);
-        it.head = unit / it.parts, it.part = unit - it.head * it.parts, it.row0 = tile * kRowTile;
+        unit_and_tile(x - first_item, p.Hkv * it.parts, tiles, unit, tile);
+        unit = __builtin_amdgcn_readfirstlane(unit), tile = __builtin_amdgcn_readfirstlane(tile);
+        it.head = __builtin_amdgcn_readfirstlane(quick_div(unit, it.parts)), it.part = unit - it.head * it.parts, it.row0 = tile * kRowTile;
         // the key tiles of this row tile: no row of it sees further than its last one
-        const int end = min(it.row0 + kRowTile, it.rows), short_ = it.rows < kRowTile;
-        const int see = p.causal ? min(it.own_keys, it.own_keys - it.n_tok + (end - 1) / p.g + 1) : it.own_keys;
-        const int first = it.stacked || !short_ ? 0 : plan.prefix_tiles;
+        const int end = min(it.row0 + kRowTile, it.rows);
+        const int see = p.causal ? min(it.own_keys, it.own_keys - it.n_tok + div_group(p, end - 1) + 1) : it.own_keys;
+        const int first = it.stacked || it.rows >= kRowTile ? 0 : plan.prefix_tiles;
         const int last = it.stacked ? plan.prefix_tiles : plan.prefix_tiles + (max(see, 0) + TK - 1) / TK;
         it.before = first > 0 ? plan.prefix_parts : 0;  // (parts that P items add in front of this item's)
-        it.u0 = first + (int)((int64_t)(last - first) * it.part / it.parts);
-        it.n_tiles = first + (int)((int64_t)(last - first) * (it.part + 1) / it.parts) - it.u0;
+        const int each = __builtin_amdgcn_readfirstlane(quick_div(last - first, it.parts)), over = last - first - each * it.parts;
+        it.u0 = first + it.part * each + min(it.part, over);
+        it.n_tiles = each + (it.part < over ? 1 : 0);
         few = end - it.row0 <= 16 * CFG::kFewBlocks;
         auto token = [&](int off) -> int {
-            const int t = min(it.row0 + off, it.rows - 1) / p.g;
+            const int t = div_group(p, min(it.row0 + off, it.rows - 1));
             if (!it.stacked) return tok0 + t;
-            const int o = owner_of(stacked_start, p.B, t);
-            return clamp_int(p.q_start[o], 0, p.T) + t - stacked_start[o];
+            const int o = owner_of(tab.stacked, p.B, t);
+            return tab.tok0[o] + t - tab.stacked[o];
         };
         toks[0] = token(few ? lane & 15 : (int)(threadIdx.x >> 6) * 32 + (lane & 31));
-        toks[1] = few ? token(16 + (lane & 15)) : toks[0];
+        toks[1] = few && CFG::kFewBlocks > 1 ? token(16 + (lane & 15)) : toks[0];
         __syncthreads();  // (the tables above have been read)
     }
     if (!few)

@@ -67,7 +67,7 @@ int check_cache(const fa_paged_cache* c) {
 }
 fa::CacheStrides strides_of(const int64_t (&s)[3]) { return {s[0], s[1], s[2]}; }
 
-constexpr int kMaxKeys = 1 << 30, kMaxParts = 64, kMaxBatch = 4096;
+constexpr int kMaxKeys = 1 << 30, kMaxParts = 64, kMaxBatch = 4000, kMaxGroup = 128;
 
 // What the host decides of a launch: the kernel divides the keys itself, from the lengths (SharedPlan); here are the
 // bounds that the workspace and the grid are made for.
@@ -100,9 +100,10 @@ int check_shared(int T, int B, int Hq, int Hkv, int prefix_len, int max_k_len) {
     if (T < 0 || B < 0) return fail(FA_ERR_SHAPE, "fa_forward_shared_prefix: T and B must not be negative");
     if (Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0)
         return fail(FA_ERR_SHAPE, "fa_forward_shared_prefix: the query heads must be a multiple of the cache's heads");
+    if (Hq / Hkv > kMaxGroup) return fail(FA_ERR_SHAPE, "fa_forward_shared_prefix: at most 128 query heads to a K/V head");
     if (prefix_len < 0 || prefix_len > kMaxKeys || max_k_len < 0 || max_k_len > kMaxKeys)
         return fail(FA_ERR_SEQLEN, "fa_forward_shared_prefix: lengths must be from 0 to 2^30");
-    if (B > kMaxBatch) return fail(FA_ERR_SHAPE, "fa_forward_shared_prefix: at most 4096 requests a call");
+    if (B > kMaxBatch) return fail(FA_ERR_SHAPE, "fa_forward_shared_prefix: at most 4000 requests a call");
     if ((int64_t)T * Hq > 0x7fffffffLL / 64 || (int64_t)B * Hq > 0x7fffffffLL / 64)
         return fail(FA_ERR_SHAPE, "fa_forward_shared_prefix: T * Hq or B * Hq too large");
     return FA_OK;
@@ -231,7 +232,9 @@ int fa_forward_shared_prefix(const uint16_t* dQ, int64_t q_tok, int64_t q_head, 
     p.T = T, p.B = B, p.Hkv = Hkv, p.g = Hq / Hkv, p.log2_page = log2_page, p.n_pages = cache->n_pages;
     p.prefix_len = prefix_len, p.table_width = table_width, p.causal = flags & FA_FLAG_CAUSAL;
     p.scale_log2e = scale * 1.44269504088896340736f;
-    p.slots = d.slots, p.max_prefix_parts = d.max_prefix_parts, p.max_own_parts = d.max_own_parts;
+    p.slots = d.slots, p.two_per_unit = D != 256, p.few_rows = D == 64 ? 32 : 16;
+    p.g_reciprocal = fa::group_reciprocal(p.g);
+    p.max_prefix_parts = d.max_prefix_parts, p.max_own_parts = d.max_own_parts;
     hipStream_t stream = static_cast<hipStream_t>(stream_);
     return timed(stream, elapsed_ms, [&]() -> int {
         if (dtype == FA_DTYPE_FP16)

@@ -323,7 +323,7 @@ enum { FA_DTYPE_FP16 = 0, FA_DTYPE_BF16 = 1 };
  *   Nothing of a page behind the last key is used, whatever it holds, nor a masked key or value (infinities and NaN
  * among them).  A table entry outside [0, n_pages) names no page: its keys take no part.  Lengths are clamped to what the table
  * names, q_start to [0, T].  Rows that see no key are 0; rows of dO that belong to no request keep their bytes.
- *   B is at most 4096.  max_k_len: no request holds more own keys than this as far as the host knows (it bounds the workspace;
+ *   B is at most 4000, Hq / cache->heads at most 128.  max_k_len: no request holds more own keys than this as far as the host knows (it bounds the workspace;
  * a longer request is still computed in full).  prefix_len is a host number: a captured launch keeps it.
  *   workspace: fa_shared_prefix_workspace(...) bytes, 16-byte aligned, for this call alone until it has run
  * (FA_ERR_WORKSPACE when it is too small).  Nothing is allocated, nothing waits: the call can be captured. */

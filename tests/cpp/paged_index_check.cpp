@@ -1,6 +1,8 @@
 // The index arithmetic of the paged-cache kernels (csrc/fa_paged_index.hpp), run on the CPU: every bound the kernels
 // rely on, over the values that could break it.  Exit status 0 and "ok" when all hold.
+#include <algorithm>
 #include <climits>
+#include <cmath>
 #include <cstdio>
 #include <cstdlib>
 #include <vector>
@@ -50,6 +52,25 @@ int main() {
         const int b = owner_of(sum, (int)len.size(), x);
         need(sum[b] <= x && x < sum[b + 1], "owner_of", x, b);
     }
+    // division by a reciprocal that is off by 1 ulp either way
+    const int tops[] = {0, 1, 2, 3, 7, 127, 128, 1000, 65535, 1 << 20, (1 << 24) + 1, (1 << 25) - 1, 1 << 30, INT_MAX - 1, INT_MAX};
+    for (int bb = 1; bb < 70000; bb += bb < 300 ? 1 : 977)
+        for (int a : tops)
+            for (int near : {-1, 0, 1}) {
+                const long x = (long)a / bb * bb + near;  // around the multiples, where a quotient goes wrong
+                for (long n : {(long)a, x}) {
+                    if (n < 0 || n > INT_MAX) continue;
+                    const float r = 1.0f / bb;
+                    for (float q : {r, std::nextafterf(r, 0.0f), std::nextafterf(r, 2.0f)})
+                        need(div_by((int)n, bb, q) == n / bb, "div_by", n, bb, div_by((int)n, bb, q));
+                }
+            }
+    for (int g = 2; g <= 128; ++g)
+        for (int i = 0; i < 4000; ++i) {
+            const unsigned top = (1u << 25) - 1, R = i < 2000 ? (unsigned)i * 16777u % (top + 1) / g * g + (i & 1 ? g - 1 : 0) : top - (i - 2000);
+            if ((uint64_t)R * g >= (uint64_t)1 << 32) continue;
+            need((unsigned)(((uint64_t)R * group_reciprocal(g)) >> 32) == R / g, "group_reciprocal", R, g);
+        }
     // workgroups of a launch: never more than the grid made from the bound, whatever the lengths
     std::srand(1);
     for (int trial = 0; trial < 20000; ++trial) {
@@ -58,21 +79,27 @@ int main() {
         const int most_prefix = 1 + std::rand() % 64, most_own = 1 + std::rand() % 64;
         std::vector<int> rows(B), own(B);
         long stacked = 0, total = 0;
-        float work = 0;
+        float few = 0, many = 0;
+        const int few_rows = std::rand() % 2 ? 16 : 32;
         for (int b = 0; b < B; ++b) {
             rows[b] = g * (std::rand() % 3 ? std::rand() % 4 : std::rand() % 300);
             own[b] = std::rand() % 4 ? std::rand() % 40 : std::rand() % 5000;
             total += rows[b];
             if (rows[b] < 128) stacked += rows[b];
-            work += (float)row_tiles(rows[b]) * (own[b] + (rows[b] < 128 ? 0 : prefix));
+            (rows[b] <= few_rows ? few : many) += (float)row_tiles(rows[b]) * (own[b] + (rows[b] < 128 ? 0 : prefix));
         }
-        work += (float)row_tiles(stacked) * prefix;
-        const int steps = steps_for(work, heads, slots, least);
-        need(steps >= least, "steps", trial);
-        long items = prefix > 0 ? (long)heads * row_tiles(stacked) * parts_for(prefix, steps, most_prefix) : 0;
+        (stacked <= few_rows ? few : many) += (float)row_tiles(stacked) * prefix;
+        const int steps_few = steps_for(few + 2 * many, heads, slots, least), half = (steps_few + 1) / 2, steps_many = half < least ? least : half;
+        need(steps_few >= least, "steps", trial);
+        // the stacked rows' ranges may be made as many as the slots
+        const int units = heads * row_tiles(stacked);
+        int p_parts = parts_for(prefix, stacked <= few_rows ? steps_few : steps_many, most_prefix);
+        if (units > 0 && units * p_parts < slots) p_parts = std::max(p_parts, std::min(slots / units, most_prefix));
+        long items = prefix > 0 ? (long)units * p_parts : 0;
         for (int b = 0; b < B; ++b)
             items += (long)heads * row_tiles(rows[b]) *
-                     (rows[b] < 128 ? parts_for(own[b], steps, most_own) : parts_for(prefix + own[b], steps, most_prefix + most_own));
+                     (rows[b] < 128 ? parts_for(own[b], rows[b] <= few_rows ? steps_few : steps_many, most_own)
+                                    : parts_for(prefix + own[b], steps_many, most_prefix + most_own));
         const long bound = blocks_bound(prefix > 0 ? row_tiles(total) : 0, request_tiles_bound(total, B), heads, slots);
         need(items <= bound, "blocks", trial, items, bound);
     }

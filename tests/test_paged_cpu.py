@@ -98,7 +98,7 @@ def shared(fa, cache, **change):
     (dict(dtype=2), 4), (dict(flags=2), 4), (dict(scale=float("nan")), 4), (dict(scale=float("inf")), 4), (dict(scale=0.0), 4), (dict(scale=-0.1), 4),
     (dict(scale=1e-40), 4), (dict(T=-1), 4), (dict(B=-1), 4),
     (dict(Hq=3), 4), (dict(Hq=0), 4), (dict(prefix_len=-1), 2), (dict(prefix_len=(1 << 30) + 1), 2), (dict(max_k=-1), 2),
-    (dict(T=1 << 24, Hq=4), 4), (dict(B=4097), 4), (dict(width=-1), 4), (dict(stride=3), 4), (dict(width=1 << 27, stride=1 << 27), 4), (dict(q=None), 5),
+    (dict(T=1 << 24, Hq=4), 4), (dict(B=4001), 4), (dict(Hq=258), 4), (dict(width=-1), 4), (dict(stride=3), 4), (dict(width=1 << 27, stride=1 << 27), 4), (dict(q=None), 5),
     (dict(o=None), 5), (dict(prefix=None), 5), (dict(table=None), 5), (dict(q_start=None), 5), (dict(k_len=None), 5), (dict(q=at(8)), 4),
     (dict(o_tok=-256), 4), (dict(q_head=60), 4), (dict(), 7), (dict(ws=None, ws_bytes=1 << 40), 7), (dict(ws=at(8), ws_bytes=1 << 40), 7),
 ])
