@@ -608,58 +608,66 @@ __device__ __forceinline__ void shared_many_rows(const SharedPrefixParams& p, co
     const int R = min(row0 + R_off, rows - 1), ti = div_group(p, R), hq = head * p.g + (R - ti * p.g), Hq = p.Hkv * p.g;
     const int own_limit = p.causal ? min(it.own_keys - 1, it.own_keys - it.n_tok + ti) : it.own_keys - 1;  // the last own key this row sees
 
-    // ---- transfers: this wave moves rows RPW * wave .. of each tile.  They lie on one page, whose number is uniform: lane L
-    //      holds the entry of the 16-key group group0 + L of the range, 64 groups at a time (the next 64 are loaded one
-    //      refill ahead).  Lane l fills slot l % kChunks of row l / kChunks of a piece with the chunk the swizzle maps there.
+    // ---- transfers: this wave moves rows RPW * wave .. of each tile, which lie on one page.  Lane L holds where the 16-key
+    //      group L of a run of 64 begins in K and in V (bytes from the head's first row; page 0 for a group on no page: its
+    //      scores are masked); the next run's pages are on their way meanwhile.  Lane l fills slot l % kChunks of row
+    //      l / kChunks of a piece with the chunk the swizzle maps there; the instruction's offset moves both sides, so it is taken
+    //      off the source's (rows are at least D apart: what remains is not negative).
     const unsigned ring_lds = __builtin_amdgcn_readfirstlane((unsigned)(size_t)(__attribute__((address_space(3))) char*)ring);
-    const int d_rip = lane / HD::kChunks, d_slot = lane % HD::kChunks;
+    const int d_rip = lane / HD::kChunks, d_slot = lane % HD::kChunks, kr = 2 * (int)p.ks.row, vr = 2 * (int)p.vs.row;
     unsigned k_off[PPW], v_off[PPW];
 #pragma unroll
     for (int j = 0; j < PPW; ++j) {
         const int row = RPW * wave + RPP * j + d_rip;
-        k_off[j] = (unsigned)((RPP * j + d_rip) * (int)p.ks.row * 2) + (unsigned)((d_slot ^ (row & HD::kKMask)) << 4);
-        v_off[j] = (unsigned)((RPP * j + d_rip) * (int)p.vs.row * 2) + (unsigned)((d_slot ^ ((row & HD::kVMask) << 2)) << 4);
+        k_off[j] = (unsigned)((RPP * j + d_rip) * kr) + (unsigned)((d_slot ^ (row & HD::kKMask)) << 4) - 1024u * j;
+        v_off[j] = (unsigned)((RPP * j + d_rip) * vr) + (unsigned)((d_slot ^ ((row & HD::kVMask) << 2)) << 4) - 1024u * j;
     }
-    const char* k_head = reinterpret_cast<const char*>(p.kc + head * p.ks.head);
-    const char* v_head = reinterpret_cast<const char*>(p.vc + head * p.vs.head);
-    auto load_pages = [&](int group) -> int { return page_of_group<TK>(p, it, group + lane, n_tiles * CPT); };
-    int pages = 0, pages_next = 0;
-    unsigned on_page = 0;  // CPT bits per tile sent for and not yet computed: the groups that lie on a page
+    const char* k_head = reinterpret_cast<const char*>(p.kc + head * p.ks.head) + (RPW * wave % 16) * (int64_t)kr;
+    const char* v_head = reinterpret_cast<const char*>(p.vc + head * p.vs.head) + (RPW * wave % 16) * (int64_t)vr;
+    const int n_groups = n_tiles * CPT;
+    auto load_pages = [&](int group) -> int { return page_of_group<TK>(p, it, group + lane, n_groups); };
+    int pages_next = load_pages(0), any_bad = 0;  // (a tile of an item with a group on no page takes the masked form)
+    uint64_t k_at = 0, v_at = 0;
+    auto refill = [&](int g0) {
+        const int page = max(pages_next, 0), u = u0 + (g0 + lane) / CPT;
+        const int row = ((u < it.prefix_tiles ? u : u - it.prefix_tiles) * TK + 16 * (lane % CPT)) & P1;
+        any_bad |= __builtin_amdgcn_readfirstlane((int)__any(pages_next < 0 && g0 + lane < n_groups));
+        k_at = 2 * ((int64_t)page * p.ks.page + (int64_t)row * p.ks.row);
+        v_at = 2 * ((int64_t)page * p.vs.page + (int64_t)row * p.vs.row);
+        if (g0 + 64 < n_groups) pages_next = load_pages(g0 + 64);
+    };
     struct Transfer {
         const char *k, *v;
         unsigned lds;
     };
+    auto lane64 = [](uint64_t x, int l) -> uint64_t {
+        const unsigned lo = __builtin_amdgcn_readlane((unsigned)x, l), hi = __builtin_amdgcn_readlane((unsigned)(x >> 32), l);
+        return (uint64_t)hi << 32 | lo;
+    };
     auto transfer = [&](int t) -> Transfer {
         const int g0 = t * CPT;
-        if ((g0 & 63) == 0) {
-            pages = t == 0 ? load_pages(0) : pages_next;
-            pages_next = g0 + 64 < n_tiles * CPT ? load_pages(g0 + 64) : -1;
-        }
-        on_page |= ((unsigned)(__ballot(pages >= 0) >> (g0 & 63)) & ((1u << CPT) - 1)) << (CPT * (ST - 1));
-        // (a group on no page is fetched from page 0: its scores are masked)
-        const int page = max(__builtin_amdgcn_readlane(pages, (g0 + wave * RPW / 16) & 63), 0);
-        const int u = u0 + t, row = ((u < it.prefix_tiles ? u : u - it.prefix_tiles) * TK + wave * RPW) & P1;
-        return {k_head + 2 * ((int64_t)page * p.ks.page + (int64_t)row * p.ks.row),
-                v_head + 2 * ((int64_t)page * p.vs.page + (int64_t)row * p.vs.row),
-                ring_lds + (unsigned)(t % ST) * kStage + (unsigned)(PPW * wave) * 1024u};
+        if ((g0 & 63) == 0) refill(g0);
+        const int l = (g0 + RPW * wave / 16) & 63;
+        return {k_head + lane64(k_at, l), v_head + lane64(v_at, l), ring_lds + (unsigned)(t % ST) * kStage + (unsigned)(PPW * wave) * 1024u};
     };
-    auto send_piece = [&](const Transfer& tr, auto jc) {
-        constexpr int j = decltype(jc)::value;
-        if constexpr (j < PPW)
-            dma16(tr.lds + 1024u * j, tr.k, k_off[j]);
-        else
-            dma16(tr.lds + kTile + 1024u * (j - PPW), tr.v, v_off[j - PPW]);
+    // on > 0: all lanes, else none (a step past the last transfer issues its pieces too, for the count that is waited for)
+    auto send_piece = [&](const Transfer& tr, int on, auto jc) {
+        constexpr int j = decltype(jc)::value % PPW;
+        constexpr bool val = decltype(jc)::value >= PPW;
+        const unsigned lds = tr.lds + (val ? kTile : 0), off = val ? v_off[j] : k_off[j];
+        const char* base = val ? tr.v : tr.k;
+        asm volatile(
+            "s_cmp_gt_i32 %4, 0\n\ts_cselect_b64 exec, -1, 0\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:%3\n\ts_mov_b64 exec, -1"
+            :
+            : "s"(lds), "v"(off), "s"(base), "n"(1024 * j), "s"(on)
+            : "memory", "scc");
     };
-    auto send = [&](int t) {
-        const Transfer tr = transfer(t);
-        static_for<2 * PPW>([&](auto ic) { send_piece(tr, ic); });
-    };
-
 #pragma unroll
-    for (int t = 0; t < ST - 1; ++t) {
-        if (t < n_tiles) send(t);
-        on_page >>= CPT;
-    }
+    for (int t = 0; t < ST - 1; ++t)
+        if (t < n_tiles) {
+            const Transfer tr = transfer(t);
+            static_for<2 * PPW>([&](auto ic) { send_piece(tr, 1, ic); });
+        }
 
     v8 qf[HD::kSteps];
     {
@@ -684,9 +692,25 @@ __device__ __forceinline__ void shared_many_rows(const SharedPrefixParams& p, co
         const int u = u0 + t, own = u - it.prefix_tiles;
         return (own < 0 ? p.prefix_len - 1 : own_limit) - (own < 0 ? u : own) * TK;
     };
-    constexpr unsigned kAllGroups = (1u << CPT) - 1;
-    auto needs_mask = [&](int lim, unsigned groups) -> int {
-        return __builtin_amdgcn_readfirstlane((int)(__any(lim < TK - 1) || groups != kAllGroups));
+    // tiles that need no mask for any row of the wave: all but the one that the prefix' end cuts and those from the first one
+    // that some row's limit cuts on
+    int own_from;
+    {
+        int low = own_limit;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) low = min(low, __shfl_xor(low, d));
+        own_from = it.prefix_tiles - u0 + (__builtin_amdgcn_readfirstlane(low) + 1) / TK;
+    }
+    const int cut = p.prefix_len % TK != 0 ? it.prefix_tiles - 1 - u0 : -1;
+    auto needs_mask = [&](int t) -> int { return (int)(t >= own_from) | (int)(t == cut) | any_bad; };
+    auto groups_of = [&](int t) -> unsigned {  // the tile's 16-key groups that lie on a page
+        unsigned g = (1u << CPT) - 1;
+        if (any_bad) {
+#pragma unroll 1
+            for (int c = 0; c < CPT; ++c)
+                if (__builtin_amdgcn_readfirstlane(page_of_group<TK>(p, it, t * CPT + c, n_groups)) < 0) g &= ~(1u << c);
+        }
+        return g;
     };
     auto mask_scores = [&](f32x16 (&s)[KB], int lim, unsigned groups) {
 #pragma unroll
@@ -718,8 +742,6 @@ __device__ __forceinline__ void shared_many_rows(const SharedPrefixParams& p, co
     };
 
     constexpr int NS = HD::kSteps * KB, NE = 16 * KB, NV = 2 * KB * HD::kBlocks, AHEAD = 4;
-    int lim = 0;
-    unsigned groups = kAllGroups;
     int specials = 0;  // masked tiles held infinities or NaN in V
     int masked = 0;  // (whole numbers in scalar registers: a branch on a lane mask would keep both sides' registers alive)
     // Q is waited for HERE: left pending, the waits in front of its uses would drain the loop's transfers
@@ -735,29 +757,27 @@ __device__ __forceinline__ void shared_many_rows(const SharedPrefixParams& p, co
         acc_reserve128();
     static_for<HD::kBlocks>([&](auto ic) { acc_zero16<16 * decltype(ic)::value>(); });
     if (wave_valid && n_tiles > 0) {
-        lim = limit_of(0);
-        groups = on_page & kAllGroups;
-        masked = needs_mask(lim, groups);
+        masked = needs_mask(0);
 #pragma unroll
         for (int b = 0; b < KB; ++b)
 #pragma unroll
             for (int e = 0; e < 16; ++e) s_cur[b][e] = 0.0f;
 #pragma unroll
         for (int i = 0; i < NS; ++i) s_cur[i % KB] = Elem<E>::mfma(k_frag(ring, i), qf[i / KB], s_cur[i % KB]);
-        if (masked) mask_scores(s_cur, lim, groups);
+        if (masked) mask_scores(s_cur, limit_of(0), groups_of(0));
         rescale(lane_max(s_cur));
     }
     // Step t: while the matrix pipe computes the next tile's scores, the vector ALU turns this tile's into probabilities; while
     // it multiplies those with V, the vector ALU takes the next scores' maximum.  Written out gap by gap: one MFMA, that
     // gap's share of the vector work, the operand read AHEAD MFMAs later, one piece of the step's transfer.
-    auto step = [&](int t, auto sends) {
-        constexpr bool kSend = decltype(sends)::value;  // tile t + ST - 1, into the stage of tile t - 1, which every wave has left
-        const bool more = kSend || t + 1 < n_tiles;
-        Transfer tr;
-        if constexpr (kSend) tr = transfer(t + ST - 1);
+    auto step = [&](int t, auto stage) {
+        constexpr int S = decltype(stage)::value;  // t % ST, so that the LDS reads' offsets are constants
+        const bool more = t + 1 < n_tiles;
+        const int on = n_tiles - (t + ST - 1);  // > 0: tile t + ST - 1, into the stage of tile t - 1, which every wave has left
+        const Transfer tr = transfer(t + ST - 1);
         if (wave_valid) {
-            const char* kb = ring + ((t + 1) % ST) * kStage;
-            const char* vb = ring + (t % ST) * kStage + kTile;
+            const char* kb = ring + (S + 1) % ST * kStage;
+            const char* vb = ring + S * kStage + kTile;
             v8 pf[2 * KB], kf[AHEAD], vf[AHEAD];
             float sum = 0.0f;
 #pragma unroll
@@ -771,7 +791,7 @@ __device__ __forceinline__ void shared_many_rows(const SharedPrefixParams& p, co
                 s_next[i % KB] = Elem<E>::mfma(kf[i % AHEAD], qf[i / KB], s_next[i % KB]);
                 if constexpr (i + AHEAD < NS) kf[i % AHEAD] = k_frag(kb, i + AHEAD);
                 constexpr int every = NS / (2 * PPW);
-                if constexpr (kSend && i % every == every - 1) send_piece(tr, std::integral_constant<int, i / every>{});
+                if constexpr (i % every == every - 1) send_piece(tr, on, std::integral_constant<int, i / every>{});
                 static_for<NE / NS>([&](auto jc) {
                     constexpr int e = i * (NE / NS) + decltype(jc)::value;
                     const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s_cur[e / 16][e % 16], c, -m_run));
@@ -793,10 +813,8 @@ __device__ __forceinline__ void shared_many_rows(const SharedPrefixParams& p, co
             for (int j = 0; j < 2 * KB; ++j) asm volatile("" : "+v"(pf[j]));
             asm volatile("s_nop 4" : "+v"(l_run));  // (wait states between a vector write and the MFMAs that read it)
 
-            const int lim_next = limit_of(t + 1);
-            const unsigned groups_next = (on_page >> CPT) & kAllGroups;
-            const int masked_next = needs_mask(lim_next, groups_next);
-            if (__builtin_expect(masked_next != 0, 0)) mask_scores(s_next, lim_next, groups_next);
+            const int masked_next = needs_mask(t + 1);
+            if (__builtin_expect(masked_next != 0, 0)) mask_scores(s_next, limit_of(t + 1), groups_of(t + 1));
             float mx;
             if (__builtin_expect(masked == 0, 1)) {
                 static_for<AHEAD>([&](auto ic) { vf[decltype(ic)::value] = v_frag(vb, decltype(ic)::value / HD::kBlocks, decltype(ic)::value % HD::kBlocks); });
@@ -828,24 +846,27 @@ __device__ __forceinline__ void shared_many_rows(const SharedPrefixParams& p, co
             }
             if (more) {
                 rescale(mx);
-                lim = lim_next, groups = groups_next, masked = masked_next;
+                masked = masked_next;
 #pragma unroll
                 for (int b = 0; b < KB; ++b) s_cur[b] = s_next[b];
             }
-        } else if constexpr (kSend) {
-            static_for<2 * PPW>([&](auto ic) { send_piece(tr, ic); });
+        } else {
+            static_for<2 * PPW>([&](auto ic) { send_piece(tr, on, ic); });
         }
-        on_page >>= CPT;
         // this wave's share of tile t + 2 has landed (transfers complete in order); what was sent since stays in flight
-        if constexpr (kSend)
-            asm volatile("s_waitcnt vmcnt(%0)" : : "n"((ST - 3) * 2 * PPW) : "memory");
-        else
-            wait_all_vmem();
+        asm volatile("s_waitcnt vmcnt(%0)" : : "n"((ST - 3) * 2 * PPW) : "memory");
         __syncthreads();
     };
-    int t = 0;
-    for (; t + ST - 1 < n_tiles; ++t) step(t, std::true_type{});
-    for (; t < n_tiles; ++t) step(t, std::false_type{});
+    for (int t = 0; t < n_tiles;) {
+        step(t, std::integral_constant<int, 0>{});
+        if (++t == n_tiles) break;
+        step(t, std::integral_constant<int, 1>{});
+        if (++t == n_tiles) break;
+        step(t, std::integral_constant<int, 2>{});
+        if (++t == n_tiles) break;
+        step(t, std::integral_constant<int, 3>{});
+        ++t;
+    }
 
     acc_fence();
     if (__builtin_expect(specials != 0, 0)) {
@@ -856,16 +877,16 @@ __device__ __forceinline__ void shared_many_rows(const SharedPrefixParams& p, co
 #pragma unroll 1
         for (int t = 0; t < n_tiles; ++t) {
             const int u = u0 + t, key = (u < it.prefix_tiles ? u : u - it.prefix_tiles) * TK, lim = limit_of(t);
-            unsigned groups = 0;
+            if (!needs_mask(t)) continue;
+            const unsigned groups = groups_of(t);
+            const char* v_rows = reinterpret_cast<const char*>(p.vc + head * p.vs.head);
 #pragma unroll 1
             for (int j = 0; j < kTile / 1024; ++j) {
-                const int row = RPP * j, page = __builtin_amdgcn_readfirstlane(page_of_group<TK>(p, it, t * CPT + row / 16, n_tiles * CPT));
-                groups |= page >= 0 ? 1u << (row / 16) : 0u;
-                const char* vb = v_head + 2 * ((int64_t)max(page, 0) * p.vs.page + (int64_t)((key + row) & P1) * p.vs.row);
+                const int row = RPP * j, page = __builtin_amdgcn_readfirstlane(page_of_group<TK>(p, it, t * CPT + row / 16, n_groups));
+                const char* vb = v_rows + 2 * ((int64_t)max(page, 0) * p.vs.page + (int64_t)((key + row) & P1) * p.vs.row);
                 dma16(mine_lds + 1024u * j, vb, (unsigned)(d_rip * (int)p.vs.row * 2) + (unsigned)((d_slot ^ (((row + d_rip) & HD::kVMask) << 2)) << 4));
             }
             wait_all_vmem();
-            if (!needs_mask(lim, groups)) continue;
             v8 sees[2 * KB];  // 1 where the row sees the key
 #pragma unroll
             for (int kk = 0; kk < 2 * KB; ++kk)
@@ -984,6 +1005,10 @@ __device__ __forceinline__ void shared_prefix_body(const SharedPrefixParams& p) 
         const int each = __builtin_amdgcn_readfirstlane(quick_div(last - first, it.parts)), over = last - first - each * it.parts;
         it.u0 = first + it.part * each + min(it.part, over);
         it.n_tiles = each + (it.part < over ? 1 : 0);
+        // (the same in every lane, though some came through the vector ALU)
+        it.parts = __builtin_amdgcn_readfirstlane(it.parts), it.part = __builtin_amdgcn_readfirstlane(it.part);
+        it.before = __builtin_amdgcn_readfirstlane(it.before), it.rows = __builtin_amdgcn_readfirstlane(it.rows);
+        it.u0 = __builtin_amdgcn_readfirstlane(it.u0), it.n_tiles = __builtin_amdgcn_readfirstlane(it.n_tiles);
         few = end - it.row0 <= 16 * CFG::kFewBlocks;
         auto token = [&](int off) -> int {
             const int t = div_group(p, min(it.row0 + off, it.rows - 1));

@@ -61,6 +61,8 @@ int check_cache(const fa_paged_cache* c) {
     if (!aligned16({c->k, c->v}) ||
         !whole_pieces({c->k_strides[0], c->k_strides[1], c->k_strides[2], c->v_strides[0], c->v_strides[1], c->v_strides[2]}))
         return fail(FA_ERR_SHAPE, "paged cache: k and v must be 16-byte aligned, strides multiples of 8 elements");
+    if (c->k_strides[2] < c->head_dim || c->v_strides[2] < c->head_dim)
+        return fail(FA_ERR_SHAPE, "paged cache: rows must not overlap");
     if (c->k_strides[2] > (1 << 25) || c->v_strides[2] > (1 << 25))  // (the lanes' offsets within 16 rows are 32-bit)
         return fail(FA_ERR_SHAPE, "paged cache: row strides must be at most 2^25 elements");
     return FA_OK;

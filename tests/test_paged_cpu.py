@@ -55,7 +55,7 @@ def test_plan_refusals(fa, change, status):
 CACHE_REFUSALS = [
     (dict(k=None), 5), (dict(v=None), 5), (dict(head_dim=96), 3), (dict(head_dim=0), 3), (dict(heads=0), 4), (dict(n_pages=0), 4),
     (dict(page_size=8), 4), (dict(page_size=48), 4), (dict(k=at(8)), 4), (dict(v=at(2)), 4), (dict(k_strides=(2048, 1024, 60)), 4),
-    (dict(v_strides=(2048, -1024, 64)), 4),
+    (dict(v_strides=(2048, -1024, 64)), 4), (dict(k_strides=(2048, 1024, 56)), 4), (dict(k_strides=(2048, 1024, 1 << 26)), 4),
 ]
 
 
