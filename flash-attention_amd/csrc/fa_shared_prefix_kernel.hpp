@@ -40,7 +40,7 @@ struct SharedPrefixParams {
     int T, B, Hkv, g, log2_page, n_pages, prefix_len, table_width, causal;
     float scale_log2e;
     int slots, two_per_unit;        // workgroups that the chip holds at a time; whether two share a compute unit
-    int few_rows;                   // up to this many rows take the form for few
+    int few_rows, few_tile, log2_few_tile;  // up to this many rows take the form for few, so many at a time
     unsigned g_reciprocal;          // 2^32 / g, rounded up
     int max_prefix_parts, max_own_parts;
 };
@@ -184,6 +184,13 @@ __device__ __forceinline__ int div_group(const SharedPrefixParams& p, int R) { r
 
 __device__ __forceinline__ int quick_parts(int tiles, int steps, int most) { return max(1, min(quick_div(tiles + (steps >> 1), steps), most)); }
 
+// Up to few_rows rows are taken few_tile at a time (each tile reads the keys again, from the L2: cheaper than the form for
+// many rows, in which one wave of four would compute), more 128 at a time.
+__device__ __forceinline__ int tile_rows(const SharedPrefixParams& p, int rows) { return rows <= p.few_rows ? p.few_tile : kRowTile; }
+__device__ __forceinline__ int tiles_of(const SharedPrefixParams& p, int rows) {
+    return rows <= p.few_rows ? (rows + p.few_tile - 1) >> p.log2_few_tile : row_tiles(rows);
+}
+
 template <int TK>
 __device__ __forceinline__ int request_parts(const SharedPrefixParams& p, const SharedPlan& s, int rows, int keys) {
     const int own = (keys + TK - 1) / TK;
@@ -221,14 +228,14 @@ __device__ __forceinline__ int shared_plan(const SharedPrefixParams& p, SharedPl
                     many += (float)row_tiles(rows) * (float)(own + s.prefix_tiles);
                 else if (rows > p.few_rows)
                     many += (float)own;
-                else if (rows > 0)
-                    few += (float)own;
+                else
+                    few += (float)tiles_of(p, rows) * (float)own;
             }
             tokens += __builtin_amdgcn_readlane(sum, 63);
         }
     }
     s.stacked = tokens * p.g;
-    const int p_tiles = row_tiles(s.stacked);
+    const int p_tiles = tiles_of(p, s.stacked);
     const bool p_few = s.stacked <= p.few_rows;
     few = wave_total(few), many = wave_total(many);
     const float prefix = (float)p_tiles * (float)s.prefix_tiles;
@@ -238,18 +245,17 @@ __device__ __forceinline__ int shared_plan(const SharedPrefixParams& p, SharedPl
     s.prefix_parts = 0;
     if (s.prefix_tiles > 0 && p_tiles > 0) {
         s.prefix_parts = quick_parts(s.prefix_tiles, p_few ? s.steps_few : s.steps_many, p.max_prefix_parts);
-        // Two workgroups to a unit: more than one P item a unit but fewer than two leaves units with two, which take twice as
-        // long.  One on each, beside the launch's other items, or two on each where there is little else.
+        // Two workgroups to a unit: with more P items than units some units hold two, which take nearly twice as long, and the
+        // requests' own items, which wait for memory, find no unit to share with one that computes.
         const int units = p_tiles * p.Hkv, half = p.slots >> 1;
-        if (p.two_per_unit && units * s.prefix_parts > half && units * s.prefix_parts < p.slots)
-            s.prefix_parts = max(1, min(quick_div(prefix * 4.0f >= 3.0f * (few * (1.0f / kManyCost) + many) ? p.slots : half, units), p.max_prefix_parts));
+        if (p.two_per_unit && units * s.prefix_parts > half && units * s.prefix_parts <= p.slots) s.prefix_parts = max(1, quick_div(half, units));
     }
     s.p_items = p_tiles * s.prefix_parts * p.Hkv;
     int items = s.p_items;
     for (int b0 = 0; b0 < p.B; b0 += 64) {
         const int b = b0 + lane, i = min(b, p.B - 1);
         const int rows = max(tab.tok0[i + 1] - tab.tok0[i], 0) * p.g;
-        const int n = b < p.B ? row_tiles(rows) * request_parts<TK>(p, s, rows, tab.keys[i]) * p.Hkv : 0, sum = wave_sum_up(n);
+        const int n = b < p.B ? tiles_of(p, rows) * request_parts<TK>(p, s, rows, tab.keys[i]) * p.Hkv : 0, sum = wave_sum_up(n);
         if (b < p.B) tab.items[b] = items + sum - n;
         items += __builtin_amdgcn_readlane(sum, 63);
     }
@@ -329,18 +335,6 @@ __device__ __forceinline__ void shared_few_rows(const SharedPrefixParams& p, con
     auto k_swz = [](int row) { return CH == 8 ? (row >> 1) & 7 : row & 15; };
     auto v_swz = [](int row) { return CH == 8 ? (row & 6) : (row & 7) << 1; };
 
-    int limit[RB], hq[RB];
-    v8 qf[RB][D / 32];
-#pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-        const int R = min(it.row0 + 16 * rb + r16, it.rows - 1), ti = div_group(p, R);
-        hq[rb] = it.head * p.g + (R - ti * p.g);
-        limit[rb] = p.causal ? min(it.own_keys - 1, it.own_keys - it.n_tok + ti) : it.own_keys - 1;
-        const uint16_t* qr = p.q + toks[rb] * p.q_tok + hq[rb] * p.q_head + q4 * 8;
-#pragma unroll
-        for (int ks = 0; ks < D / 32; ++ks) qf[rb][ks] = *reinterpret_cast<const v8*>(qr + ks * 32);
-    }
-
     const int all = it.n_tiles * CPT, g0 = (int)((int64_t)all * wave / 4), n = (int)((int64_t)all * (wave + 1) / 4) - g0;
     char* mine = ring + wave * N * 2 * kGran;
     const unsigned lds = __builtin_amdgcn_readfirstlane((unsigned)(size_t)(__attribute__((address_space(3))) char*)mine);
@@ -357,6 +351,18 @@ __device__ __forceinline__ void shared_few_rows(const SharedPrefixParams& p, con
     int pages = page_of_group<TK>(p, it, g0 + lane, g0 + n), pages_next = -1;
     if (n > 64) pages_next = page_of_group<TK>(p, it, g0 + 64 + lane, g0 + n);
     int page_k = 0, row_k = 0;
+    int limit[RB], hq[RB];
+    v8 qf[RB][D / 32];
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+        const int R = min(it.row0 + 16 * rb + r16, it.rows - 1), ti = div_group(p, R);
+        hq[rb] = it.head * p.g + (R - ti * p.g);
+        limit[rb] = p.causal ? min(it.own_keys - 1, it.own_keys - it.n_tok + ti) : it.own_keys - 1;
+        const uint16_t* qr = p.q + toks[rb] * p.q_tok + hq[rb] * p.q_head + q4 * 8;
+#pragma unroll
+        for (int ks = 0; ks < D / 32; ++ks) qf[rb][ks] = *reinterpret_cast<const v8*>(qr + ks * 32);
+    }
+
     auto send_k = [&](int i) {
         if ((i & 63) == 0 && i > 0) {
             pages = pages_next;
@@ -627,6 +633,14 @@ __device__ __forceinline__ void shared_many_rows(const SharedPrefixParams& p, co
     const int n_groups = n_tiles * CPT;
     auto load_pages = [&](int group) -> int { return page_of_group<TK>(p, it, group + lane, n_groups); };
     int pages_next = load_pages(0), any_bad = 0;  // (a tile of an item with a group on no page takes the masked form)
+    // (Q's loads go out beside the first pages')
+    v8 qf[HD::kSteps];
+    {
+        const uint16_t* qr = p.q + tok * p.q_tok + hq * p.q_head + geo.hh * 8;
+#pragma unroll
+        for (int ks = 0; ks < HD::kSteps; ++ks) qf[ks] = *reinterpret_cast<const v8*>(qr + ks * 16);
+    }
+
     uint64_t k_at = 0, v_at = 0;
     auto refill = [&](int g0) {
         const int page = max(pages_next, 0), u = u0 + (g0 + lane) / CPT;
@@ -668,13 +682,6 @@ __device__ __forceinline__ void shared_many_rows(const SharedPrefixParams& p, co
             const Transfer tr = transfer(t);
             static_for<2 * PPW>([&](auto ic) { send_piece(tr, 1, ic); });
         }
-
-    v8 qf[HD::kSteps];
-    {
-        const uint16_t* qr = p.q + tok * p.q_tok + hq * p.q_head + geo.hh * 8;
-#pragma unroll
-        for (int ks = 0; ks < HD::kSteps; ++ks) qf[ks] = *reinterpret_cast<const v8*>(qr + ks * 16);
-    }
 
     f32x16 s_cur[KB], s_next[KB];
     float m_run = -1e30f, l_run = 0.0f;
@@ -981,7 +988,7 @@ __device__ __forceinline__ void shared_prefix_body(const SharedPrefixParams& p) 
         it.own_keys = it.n_tok = 0;
         it.own_table = nullptr;
         if (it.stacked) {
-            it.rows = plan.stacked, it.parts = plan.prefix_parts, tiles = row_tiles(plan.stacked);
+            it.rows = plan.stacked, it.parts = plan.prefix_parts, tiles = tiles_of(p, plan.stacked);
         } else {
             const int b = last_at_most(tab.items, p.B, x);
             tok0 = __builtin_amdgcn_readfirstlane(tab.tok0[b]);
@@ -989,15 +996,15 @@ __device__ __forceinline__ void shared_prefix_body(const SharedPrefixParams& p) 
             it.own_keys = __builtin_amdgcn_readfirstlane(tab.keys[b]);
             first_item = __builtin_amdgcn_readfirstlane(tab.items[b]);
             it.rows = it.n_tok * p.g;
-            tiles = row_tiles(it.rows);
+            tiles = tiles_of(p, it.rows);
             it.parts = __builtin_amdgcn_readfirstlane(request_parts<TK>(p, plan, it.rows, it.own_keys));
             it.own_table = p.block_table + b * p.table_stride;
         }
         unit_and_tile(x - first_item, p.Hkv * it.parts, tiles, unit, tile);
         unit = __builtin_amdgcn_readfirstlane(unit), tile = __builtin_amdgcn_readfirstlane(tile);
-        it.head = __builtin_amdgcn_readfirstlane(quick_div(unit, it.parts)), it.part = unit - it.head * it.parts, it.row0 = tile * kRowTile;
+        it.head = __builtin_amdgcn_readfirstlane(quick_div(unit, it.parts)), it.part = unit - it.head * it.parts, it.row0 = tile * tile_rows(p, it.rows);
         // the key tiles of this row tile: no row of it sees further than its last one
-        const int end = min(it.row0 + kRowTile, it.rows);
+        const int end = min(it.row0 + tile_rows(p, it.rows), it.rows);
         const int see = p.causal ? min(it.own_keys, it.own_keys - it.n_tok + div_group(p, end - 1) + 1) : it.own_keys;
         const int first = it.stacked || it.rows >= kRowTile ? 0 : plan.prefix_tiles;
         const int last = it.stacked ? plan.prefix_tiles : plan.prefix_tiles + (max(see, 0) + TK - 1) / TK;
@@ -1009,7 +1016,7 @@ __device__ __forceinline__ void shared_prefix_body(const SharedPrefixParams& p) 
         it.parts = __builtin_amdgcn_readfirstlane(it.parts), it.part = __builtin_amdgcn_readfirstlane(it.part);
         it.before = __builtin_amdgcn_readfirstlane(it.before), it.rows = __builtin_amdgcn_readfirstlane(it.rows);
         it.u0 = __builtin_amdgcn_readfirstlane(it.u0), it.n_tiles = __builtin_amdgcn_readfirstlane(it.n_tiles);
-        few = end - it.row0 <= 16 * CFG::kFewBlocks;
+        few = it.rows <= p.few_rows;
         auto token = [&](int off) -> int {
             const int t = div_group(p, min(it.row0 + off, it.rows - 1));
             if (!it.stacked) return tok0 + t;
@@ -1022,7 +1029,7 @@ __device__ __forceinline__ void shared_prefix_body(const SharedPrefixParams& p) 
     }
     if (!few)
         shared_many_rows<E, D>(p, it, toks[0], ring);
-    else if (CFG::kFewBlocks == 1 || min(it.rows - it.row0, kRowTile) <= 16)
+    else if (CFG::kFewBlocks == 1 || it.rows - it.row0 <= 16)
         shared_few_rows<E, D, 1>(p, it, toks, ring);
     else
         shared_few_rows<E, D, CFG::kFewBlocks>(p, it, toks, ring);

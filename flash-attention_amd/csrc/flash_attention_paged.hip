@@ -90,7 +90,8 @@ Bounds bounds_of(int T, int B, int Hkv, int g, int D, int prefix_len, int max_k_
     d.max_prefix_parts = prefix_len > 0 ? within(up(2 * d.slots, up(rows, 128) * Hkv), 1, within(up(prefix_len, 128), 1, kMaxParts)) : 0;
     d.max_own_parts = within(up(2 * d.slots, (int64_t)B * Hkv), 4, kMaxParts);
     d.max_own_parts = within(up(max_k_len, 128), 1, d.max_own_parts);
-    const int64_t p_tiles = prefix_len > 0 ? fa::row_tiles(rows) : 0, r_tiles = fa::request_tiles_bound(rows, B);
+    // (a batch or a request of few rows has two tiles at most, where 128 rows would be one)
+    const int64_t p_tiles = prefix_len > 0 ? fa::row_tiles(rows) + 1 : 0, r_tiles = fa::request_tiles_bound(rows, B) + B;
     d.blocks = std::min(Hkv * (p_tiles * d.max_prefix_parts + r_tiles * d.parts()), fa::blocks_bound(p_tiles, r_tiles, Hkv, d.slots));
     return d;
 }
@@ -234,7 +235,7 @@ int fa_forward_shared_prefix(const uint16_t* dQ, int64_t q_tok, int64_t q_head, 
     p.T = T, p.B = B, p.Hkv = Hkv, p.g = Hq / Hkv, p.log2_page = log2_page, p.n_pages = cache->n_pages;
     p.prefix_len = prefix_len, p.table_width = table_width, p.causal = flags & FA_FLAG_CAUSAL;
     p.scale_log2e = scale * 1.44269504088896340736f;
-    p.slots = d.slots, p.two_per_unit = D != 256, p.few_rows = D == 64 ? 32 : 16;
+    p.slots = d.slots, p.two_per_unit = D != 256, p.few_tile = D == 64 ? 32 : 16, p.log2_few_tile = D == 64 ? 5 : 4, p.few_rows = 2 * p.few_tile;
     p.g_reciprocal = fa::group_reciprocal(p.g);
     p.max_prefix_parts = d.max_prefix_parts, p.max_own_parts = d.max_own_parts;
     hipStream_t stream = static_cast<hipStream_t>(stream_);

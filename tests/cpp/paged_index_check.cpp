@@ -80,27 +80,28 @@ int main() {
         std::vector<int> rows(B), own(B);
         long stacked = 0, total = 0;
         float few = 0, many = 0;
-        const int few_rows = std::rand() % 2 ? 16 : 32;
+        const int few_tile = std::rand() % 2 ? 16 : 32, few_rows = 2 * few_tile;
+        auto tiles = [&](long r) { return r <= few_rows ? (int)((r + few_tile - 1) / few_tile) : row_tiles(r); };
         for (int b = 0; b < B; ++b) {
             rows[b] = g * (std::rand() % 3 ? std::rand() % 4 : std::rand() % 300);
             own[b] = std::rand() % 4 ? std::rand() % 40 : std::rand() % 5000;
             total += rows[b];
             if (rows[b] < 128) stacked += rows[b];
-            (rows[b] <= few_rows ? few : many) += (float)row_tiles(rows[b]) * (own[b] + (rows[b] < 128 ? 0 : prefix));
+            (rows[b] <= few_rows ? few : many) += (float)tiles(rows[b]) * (own[b] + (rows[b] < 128 ? 0 : prefix));
         }
-        (stacked <= few_rows ? few : many) += (float)row_tiles(stacked) * prefix;
+        (stacked <= few_rows ? few : many) += (float)tiles(stacked) * prefix;
         const int steps_few = steps_for(few + 2 * many, heads, slots, least), half = (steps_few + 1) / 2, steps_many = half < least ? least : half;
         need(steps_few >= least, "steps", trial);
         // the stacked rows' ranges may be made as many as the slots
-        const int units = heads * row_tiles(stacked);
+        const int units = heads * tiles(stacked);
         int p_parts = parts_for(prefix, stacked <= few_rows ? steps_few : steps_many, most_prefix);
         if (units > 0 && units * p_parts < slots) p_parts = std::max(p_parts, std::min(slots / units, most_prefix));
         long items = prefix > 0 ? (long)units * p_parts : 0;
         for (int b = 0; b < B; ++b)
-            items += (long)heads * row_tiles(rows[b]) *
+            items += (long)heads * tiles(rows[b]) *
                      (rows[b] < 128 ? parts_for(own[b], rows[b] <= few_rows ? steps_few : steps_many, most_own)
                                     : parts_for(prefix + own[b], steps_many, most_prefix + most_own));
-        const long bound = blocks_bound(prefix > 0 ? row_tiles(total) : 0, request_tiles_bound(total, B), heads, slots);
+        const long bound = blocks_bound(prefix > 0 ? row_tiles(total) + 1 : 0, request_tiles_bound(total, B) + B, heads, slots);
         need(items <= bound, "blocks", trial, items, bound);
     }
     std::printf("ok\n");
