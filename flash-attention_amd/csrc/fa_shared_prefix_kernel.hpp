@@ -664,23 +664,25 @@ __device__ __forceinline__ void shared_many_rows(const SharedPrefixParams& p, co
         const int l = (g0 + RPW * wave / 16) & 63;
         return {k_head + lane64(k_at, l), v_head + lane64(v_at, l), ring_lds + (unsigned)(t % ST) * kStage + (unsigned)(PPW * wave) * 1024u};
     };
-    // on > 0: all lanes, else none (a step past the last transfer issues its pieces too, for the count that is waited for)
-    auto send_piece = [&](const Transfer& tr, int on, auto jc) {
-        constexpr int j = decltype(jc)::value % PPW;
-        constexpr bool val = decltype(jc)::value >= PPW;
-        const unsigned lds = tr.lds + (val ? kTile : 0), off = val ? v_off[j] : k_off[j];
+    // Two pieces of K (first half of the indices) or of V in one go.  on > 0: all lanes, else none (a step past the last transfer
+    // issues its pieces too, for the count that is waited for).
+    auto send_pair = [&](const Transfer& tr, int on, auto jc) {
+        constexpr int j = 2 * decltype(jc)::value % PPW;
+        constexpr bool val = 2 * decltype(jc)::value >= PPW;
+        const unsigned lds = tr.lds + (val ? kTile : 0), off0 = val ? v_off[j] : k_off[j], off1 = val ? v_off[j + 1] : k_off[j + 1];
         const char* base = val ? tr.v : tr.k;
         asm volatile(
-            "s_cmp_gt_i32 %4, 0\n\ts_cselect_b64 exec, -1, 0\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 offset:%3\n\ts_mov_b64 exec, -1"
+            "s_cmp_gt_i32 %6, 0\n\ts_cselect_b64 exec, -1, 0\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %3 offset:%4\n\t"
+            "global_load_lds_dwordx4 %2, %3 offset:%5\n\ts_mov_b64 exec, -1"
             :
-            : "s"(lds), "v"(off), "s"(base), "n"(1024 * j), "s"(on)
+            : "s"(lds), "v"(off0), "v"(off1), "s"(base), "n"(1024 * j), "n"(1024 * (j + 1)), "s"(on)
             : "memory", "scc");
     };
 #pragma unroll
     for (int t = 0; t < ST - 1; ++t)
         if (t < n_tiles) {
             const Transfer tr = transfer(t);
-            static_for<2 * PPW>([&](auto ic) { send_piece(tr, 1, ic); });
+            static_for<PPW>([&](auto ic) { send_pair(tr, 1, ic); });
         }
 
     f32x16 s_cur[KB], s_next[KB];
@@ -797,8 +799,8 @@ __device__ __forceinline__ void shared_many_rows(const SharedPrefixParams& p, co
                 constexpr int i = decltype(ic)::value;
                 s_next[i % KB] = Elem<E>::mfma(kf[i % AHEAD], qf[i / KB], s_next[i % KB]);
                 if constexpr (i + AHEAD < NS) kf[i % AHEAD] = k_frag(kb, i + AHEAD);
-                constexpr int every = NS / (2 * PPW);
-                if constexpr (i % every == every - 1) send_piece(tr, on, std::integral_constant<int, i / every>{});
+                constexpr int every = NS / PPW;
+                if constexpr (i % every == every - 1) send_pair(tr, on, std::integral_constant<int, i / every>{});
                 static_for<NE / NS>([&](auto jc) {
                     constexpr int e = i * (NE / NS) + decltype(jc)::value;
                     const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s_cur[e / 16][e % 16], c, -m_run));
@@ -858,7 +860,7 @@ __device__ __forceinline__ void shared_many_rows(const SharedPrefixParams& p, co
                 for (int b = 0; b < KB; ++b) s_cur[b] = s_next[b];
             }
         } else {
-            static_for<2 * PPW>([&](auto ic) { send_piece(tr, on, ic); });
+            static_for<PPW>([&](auto ic) { send_pair(tr, on, ic); });
         }
         // this wave's share of tile t + 2 has landed (transfers complete in order); what was sent since stays in flight
         asm volatile("s_waitcnt vmcnt(%0)" : : "n"((ST - 3) * 2 * PPW) : "memory");
