@@ -17,7 +17,7 @@
 namespace fa {
 
 constexpr int kMinLog2Page = 4, kMaxLog2Page = 16;
-constexpr int kMaxPlanRequests = 5120;  // three sums per request in a workgroup's LDS: 61 of the 64 KB a launch may ask for
+constexpr int kMaxPlanRequests = 5120;  // four numbers per request in a workgroup's LDS, five requests per thread
 
 // Element strides of one cache tensor.
 struct CacheStrides {

@@ -17,6 +17,7 @@
 #pragma once
 #include "fa_fwd_general_kernel.hpp"
 #include "fa_fwd_ring_kernel.hpp"  // wait_all_vmem
+#include "fa_cache_kernels.hpp"  // wave_sum_up
 #include "fa_owned_acc.hpp"
 #include "fa_paged_index.hpp"
 
@@ -156,18 +157,8 @@ struct SharedTables {
 };
 
 template <int CTRL, int ROWS>
-__device__ __forceinline__ int dpp_int(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, true); }
-template <int CTRL, int ROWS>
-__device__ __forceinline__ float dpp_float(float v) { return __builtin_bit_cast(float, dpp_int<CTRL, ROWS>(__builtin_bit_cast(int, v))); }
-// Inclusive sum over the wave: within rows of 16 lanes, then row ends into the rows above.
-__device__ __forceinline__ int wave_sum_up(int v) {
-    v += dpp_int<0x111, 0xf>(v);
-    v += dpp_int<0x112, 0xf>(v);
-    v += dpp_int<0x114, 0xf>(v);
-    v += dpp_int<0x118, 0xf>(v);
-    v += dpp_int<0x142, 0xa>(v);
-    v += dpp_int<0x143, 0xc>(v);
-    return v;
+__device__ __forceinline__ float dpp_float(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, true));
 }
 __device__ __forceinline__ float wave_total(float v) {
     v += dpp_float<0x111, 0xf>(v);

@@ -138,7 +138,7 @@ int fa_cache_plan(const int* k_len, const int* n_new, int* block_table, int64_t 
     const int log2_page = log2_page_of(page_size);
     if (log2_page < 0) return fail(FA_ERR_SHAPE, "fa_cache_plan: page_size must be a power of two from 16 to 65536");
     if (B <= 0 || B > fa::kMaxPlanRequests) return fail(FA_ERR_SHAPE, "fa_cache_plan: B must be from 1 to 5120");
-    if (table_width <= 0 || ((int64_t)table_width << log2_page) > kMaxKeys || (int64_t)B * table_width > (1 << 30) ||
+    if (table_width <= 0 || ((int64_t)table_width << log2_page) > kMaxKeys || (int64_t)B * table_width >= (1 << 30) ||
         table_stride < table_width)
         return fail(FA_ERR_SHAPE, "fa_cache_plan: the block table's rows must be positive, name at most 2^30 keys, and fit their stride");
     if (free_cap < 0 || free_cap > (1 << 30) || max_tokens < 0 || max_tokens > (1 << 30))
@@ -157,12 +157,16 @@ int fa_cache_plan(const int* k_len, const int* n_new, int* block_table, int64_t 
     hipStream_t stream = static_cast<hipStream_t>(stream_);
     fa::CachePlanParams p{k_len, n_new, block_table, table_stride, free_pages, free_count, q_start, k_len_out, slots, counts,
                           B, table_width, log2_page, free_cap, max_tokens};
-    constexpr int threads = 1024;
-    int64_t blocks = (std::max(max_tokens, B) + 4 * threads - 1) / (4 * threads);
-    if (blocks > 64) blocks = 64;
+    // small steps: a smaller workgroup's rounds of sums are quicker; large ones: a thread or two per token and request
+    const bool small = B <= 256;
+    const int threads = small ? 256 : 1024;
+    int64_t blocks = (std::max(max_tokens, B) + threads - 1) / threads;
+    if (blocks > 256) blocks = 256;
     return timed(stream, elapsed_ms, [&]() -> int {
-        hipLaunchKernelGGL(fa::fa_cache_plan_kernel<threads>, dim3((unsigned)blocks), dim3(threads), (size_t)3 * (B + 1) * sizeof(int),
-                           stream, p);
+        if (small)
+            hipLaunchKernelGGL(fa::fa_cache_plan_kernel<256>, dim3((unsigned)blocks), dim3(256), 0, stream, p);
+        else
+            hipLaunchKernelGGL(fa::fa_cache_plan_kernel<1024>, dim3((unsigned)blocks), dim3(1024), 0, stream, p);
         return hip_ok(hipGetLastError(), "fa_cache_plan_kernel");
     });
 }
