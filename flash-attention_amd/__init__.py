@@ -454,30 +454,47 @@ def make_cache_plan(B: int, max_tokens: int, device) -> CachePlan:
     return CachePlan(*(torch.empty(n, dtype=torch.int32, device=device) for n in (B + 1, B, max_tokens, 2)))
 
 
-def _on_device(index: int):
-    """The current device for a launch on GPU ``index``: nothing to do when it is that already."""
+def _raw_stream(torch, stream, index: int) -> int:
+    """Handle of ``stream`` (a torch stream, a handle, or None: the current one of GPU ``index``)."""
+    if stream is None:
+        return torch._C._cuda_getCurrentRawStream(index)
+    return stream if isinstance(stream, int) else stream.cuda_stream
+
+
+def _allocating_for(torch, stream, device):
+    """What a call on ``stream`` allocates (and zeroes) belongs to that stream."""
     import contextlib
 
-    import torch
+    if stream is None:
+        return contextlib.nullcontext()
+    return torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device) if isinstance(stream, int) else stream)
 
-    return contextlib.nullcontext() if torch.cuda.current_device() == index else torch.cuda.device(index)
+
+def _run_on(torch, index: int, call, *args, timed: bool = False) -> float:
+    """Calls a library function, its elapsed_ms argument last, with GPU ``index`` current; raises on its errors."""
+    ms = ct.c_float(0.0) if timed else None
+    if torch._C._cuda_getDevice() == index:
+        rc = call(*args, ct.byref(ms) if timed else None)
+    else:
+        with torch.cuda.device(index):
+            rc = call(*args, ct.byref(ms) if timed else None)
+    if rc:
+        _check(rc)
+    return ms.value if timed else 0.0
 
 
-def _int_tensor(t, name: str, index: int, n: int) -> int:
+def _int_tensor(torch, t, name: str, index: int, n: int) -> int:
     """Address of a contiguous int32 tensor of ``n`` entries on GPU ``index``."""
-    import torch
-
-    if t.dtype != torch.int32 or t.get_device() != index or t.numel() != n or not t.is_contiguous():
+    if t.dtype is not torch.int32 or t.get_device() != index or t.numel() != n or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 tensor of {n} entries on the call's GPU")
     return t.data_ptr()
 
 
-def _table(t, name: str, index: int, rows: int):
-    import torch
-
-    if t.dim() != 2 or t.dtype != torch.int32 or t.get_device() != index or t.shape[0] != rows or (t.shape[1] > 1 and t.stride(1) != 1):
+def _table(torch, t, name: str, index: int, rows: int):
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 2 or t.dtype is not torch.int32 or t.get_device() != index or shape[0] != rows or (shape[1] > 1 and stride[1] != 1):
         raise ValueError(f"{name} must be an int32 tensor [{rows}, width] with contiguous rows on the call's GPU")
-    return t.data_ptr(), max(t.stride(0), t.shape[1]) if rows == 1 else t.stride(0), t.shape[1]
+    return t.data_ptr(), max(stride[0], shape[1]) if rows == 1 else stride[0], shape[1]
 
 
 def cache_plan(k_len, n_new, block_table, free_pages, free_count, page_size: int, max_tokens: int = None, out: CachePlan = None,
@@ -494,29 +511,27 @@ def cache_plan(k_len, n_new, block_table, free_pages, free_count, page_size: int
     if out is None:
         if max_tokens is None:
             raise ValueError("cache_plan() needs max_tokens or out")
-        out = make_cache_plan(B, max_tokens, k_len.device)
+        with _allocating_for(torch, stream, k_len.device):
+            out = make_cache_plan(B, max_tokens, k_len.device)
     elif max_tokens is not None and max_tokens != out.slots.numel():
         raise ValueError("max_tokens must be the size of out.slots")
-    if stream is None:
-        stream = torch.cuda.current_stream(dev)
-    table, stride, width = _table(block_table, "block_table", dev, B)
+    table, stride, width = _table(torch, block_table, "block_table", dev, B)
     max_tokens, cap = out.slots.numel(), free_pages.numel()
-    ms = ct.c_float(0.0)
-    with _on_device(dev):
-        _check(lib().fa_cache_plan(
-            _int_tensor(k_len, "k_len", dev, B), _int_tensor(n_new, "n_new", dev, B), table, stride,
-            _int_tensor(free_pages, "free_pages", dev, cap), _int_tensor(free_count, "free_count", dev, 1),
-            _int_tensor(out.q_start, "out.q_start", dev, B + 1), _int_tensor(out.k_len, "out.k_len", dev, B),
-            _int_tensor(out.slots, "out.slots", dev, max_tokens), _int_tensor(out.counts, "out.counts", dev, 2),
-            B, width, page_size, cap, max_tokens, _stream_handle(stream), ct.byref(ms) if timed else None))
-    return (out, float(ms.value)) if timed else out
+    ms = _run_on(
+        torch, dev, lib().fa_cache_plan, _int_tensor(torch, k_len, "k_len", dev, B), _int_tensor(torch, n_new, "n_new", dev, B), table, stride,
+        _int_tensor(torch, free_pages, "free_pages", dev, cap), _int_tensor(torch, free_count, "free_count", dev, 1),
+        _int_tensor(torch, out.q_start, "out.q_start", dev, B + 1), _int_tensor(torch, out.k_len, "out.k_len", dev, B),
+        _int_tensor(torch, out.slots, "out.slots", dev, max_tokens), _int_tensor(torch, out.counts, "out.counts", dev, 2),
+        B, width, page_size, cap, max_tokens, _raw_stream(torch, stream, dev), timed=timed)
+    return (out, ms) if timed else out
 
 
 def _token_rows(t, name: str, heads, cache: "PagedCache"):
-    if t.dim() != 3 or t.dtype != cache.dtype or t.get_device() != cache.device_index or t.shape[2] != cache.head_dim or \
-            (heads is not None and t.shape[1] != heads) or (t.stride(2) != 1 and t.numel()):
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 3 or t.dtype is not cache.dtype or t.get_device() != cache.device_index or shape[2] != cache.head_dim or \
+            (heads is not None and shape[1] != heads) or (stride[2] != 1 and t.numel()):
         raise ValueError(f"{name} must be [T, heads, {cache.head_dim}] with contiguous rows, of the cache's dtype and GPU")
-    return t.data_ptr(), t.stride(0), t.stride(1)
+    return t.data_ptr(), stride[0], stride[1]
 
 
 def cache_write(k, v, cache: PagedCache, slots, stream=None, timed: bool = False):
@@ -527,22 +542,22 @@ def cache_write(k, v, cache: PagedCache, slots, stream=None, timed: bool = False
     T, dev = k.shape[0], cache.device_index
     if v.shape != k.shape:
         raise ValueError("k and v must share one [T, Hkv, D] shape")
-    if slots.numel() < T:
+    n = slots.numel()
+    if n < T:
         raise ValueError("slots must name a slot for every token")
     kp, kt, kh = _token_rows(k, "k", cache.heads, cache)
     vp, vt, vh = _token_rows(v, "v", cache.heads, cache)
-    if stream is None:
-        stream = torch.cuda.current_stream(dev)
-    ms = ct.c_float(0.0)
-    with _on_device(dev):
-        _check(lib().fa_cache_write(kp, vp, kt, kh, vt, vh, cache.ref, _int_tensor(slots, "slots", dev, slots.numel()), T,
-                                    _stream_handle(stream), ct.byref(ms) if timed else None))
-    return float(ms.value) if timed else None
+    ms = _run_on(torch, dev, lib().fa_cache_write, kp, vp, kt, kh, vt, vh, cache.ref, _int_tensor(torch, slots, "slots", dev, n), T,
+                 _raw_stream(torch, stream, dev), timed=timed)
+    return ms if timed else None
 
 
 @functools.lru_cache(maxsize=4096)
 def _shared_prefix_workspace(device: int, *sizes) -> int:
-    return lib().fa_shared_prefix_workspace(*sizes)
+    import torch
+
+    with torch.cuda.device(device):
+        return lib().fa_shared_prefix_workspace(*sizes)
 
 
 def attention_shared_prefix(q, cache: PagedCache, q_start, k_len, block_table, prefix_table=None, prefix_len: int = 0,
@@ -561,36 +576,35 @@ def attention_shared_prefix(q, cache: PagedCache, q_start, k_len, block_table, p
     qp, qt, qh = _token_rows(q, "q", None, cache)
     T, Hq, D = q.shape
     if out is None:
-        out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
+        with _allocating_for(torch, stream, cache.device):
+            out = torch.zeros(q.shape, dtype=q.dtype, device=q.device)
     elif out.shape != q.shape:
         raise ValueError("out must have q's shape")
     op, ot, oh = _token_rows(out, "out", Hq, cache)
     B = k_len.numel()
     if Hq % cache.heads:
         raise ValueError("q's heads must be a multiple of the cache's")
-    table, stride, width = _table(block_table, "block_table", dev, B)
+    table, stride, width = _table(torch, block_table, "block_table", dev, B)
     if prefix_len:
         if prefix_table is None or prefix_table.numel() * cache.page_size < prefix_len:
             raise ValueError("prefix_table must name the pages of prefix_len keys")
-        prefix = _int_tensor(prefix_table, "prefix_table", dev, prefix_table.numel())
+        prefix = _int_tensor(torch, prefix_table, "prefix_table", dev, prefix_table.numel())
     else:
         prefix = None
     room = width * cache.page_size
     max_k = room if max_k_len is None else max(0, min(max_k_len, room))
-    if stream is None:
-        stream = torch.cuda.current_stream(dev)
+    handle = _raw_stream(torch, stream, dev)
     n = _shared_prefix_workspace(dev, T, B, Hq, cache.heads, D, prefix_len, max_k)
-    ms = ct.c_float(0.0)
-    with _on_device(dev):
-        workspace = torch.empty(n, dtype=torch.uint8, device=q.device)
-        if isinstance(stream, int) or stream != torch.cuda.current_stream(dev):
-            workspace.record_stream(torch.cuda.ExternalStream(stream) if isinstance(stream, int) else stream)
-        _check(lib().fa_forward_shared_prefix(
-            qp, qt, qh, op, ot, oh, cache.ref, prefix, prefix_len, table, stride, width, _int_tensor(q_start, "q_start", dev, B + 1),
-            _int_tensor(k_len, "k_len", dev, B), T, B, Hq, cache.dtype_code, FLAG_CAUSAL if causal else 0,
-            D ** -0.5 if scale is None else scale, max_k, workspace.data_ptr(), n, _stream_handle(stream),
-            ct.byref(ms) if timed else None))
-    return (out, float(ms.value)) if timed else out
+    if stream is None:
+        workspace = torch.empty(n, dtype=torch.uint8, device=cache.device)
+    else:
+        with _allocating_for(torch, stream, cache.device):
+            workspace = torch.empty(n, dtype=torch.uint8, device=cache.device)
+    ms = _run_on(
+        torch, dev, lib().fa_forward_shared_prefix, qp, qt, qh, op, ot, oh, cache.ref, prefix, prefix_len, table, stride, width,
+        _int_tensor(torch, q_start, "q_start", dev, B + 1), _int_tensor(torch, k_len, "k_len", dev, B), T, B, Hq, cache.dtype_code,
+        FLAG_CAUSAL if causal else 0, D ** -0.5 if scale is None else scale, max_k, workspace.data_ptr(), n, handle, timed=timed)
+    return (out, ms) if timed else out
 
 
 def init_half(t, seed: int, stream=None) -> None:
