@@ -196,15 +196,15 @@ __device__ __forceinline__ int shared_plan(const SharedPrefixParams& p, SharedPl
     s.prefix_tiles = (p.prefix_len + TK - 1) / TK;
     int tokens = 0;
     float few = 0.0f, many = 0.0f;  // key tiles of all row tiles, per K/V head
-    for (int b0 = 0; b0 < p.B; b0 += 256) {
-        int q0[4], q1[4], k[4];
+    for (int b0 = 0; b0 < p.B; b0 += 128) {
+        int q0[2], q1[2], k[2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 2; ++i) {
             const int b = min(b0 + 64 * i + lane, p.B - 1);
             q0[i] = p.q_start[b], q1[i] = p.q_start[b + 1], k[i] = p.k_len[b];
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 2; ++i) {
             if (b0 + 64 * i >= p.B) break;
             const int b = b0 + 64 * i + lane;
             const int tok0 = clamp_int(q0[i], 0, p.T), keys = clamp_int(k[i], 0, p.table_width << p.log2_page);
@@ -231,8 +231,8 @@ __device__ __forceinline__ int shared_plan(const SharedPrefixParams& p, SharedPl
     few = wave_total(few), many = wave_total(many);
     const float prefix = (float)p_tiles * (float)s.prefix_tiles;
     (p_few ? few : many) += prefix;
-    s.steps_few = steps_for(few + (float)kManyCost * many, p.Hkv, p.slots, 128 / TK);
-    s.steps_many = max(128 / TK, (s.steps_few + kManyCost - 1) / kManyCost);
+    s.steps_few = steps_for(few + (float)kManyCost * many, p.Hkv, p.slots, 256 / TK);
+    s.steps_many = max(256 / TK, (s.steps_few + kManyCost - 1) / kManyCost);
     s.prefix_parts = 0;
     if (s.prefix_tiles > 0 && p_tiles > 0) {
         s.prefix_parts = quick_parts(s.prefix_tiles, p_few ? s.steps_few : s.steps_many, p.max_prefix_parts);
