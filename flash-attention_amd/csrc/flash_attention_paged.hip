@@ -71,8 +71,9 @@ fa::CacheStrides strides_of(const int64_t (&s)[3]) { return {s[0], s[1], s[2]}; 
 
 constexpr int kMaxKeys = 1 << 30, kMaxParts = 64, kMaxBatch = 4000, kMaxGroup = 128;
 
-// What the host decides of a launch: the kernel divides the keys itself, from the lengths (SharedPlan); here are the
-// bounds that the workspace and the grid are made for.
+// What the host decides of a launch: the kernel divides the keys itself, from the lengths (SharedPlan), which the host does
+// not know; here are the bounds that the workspace and the grid are made for.  Two workgroups share a compute unit at D = 64 and
+// 128 (64 KiB of LDS, at most 256 registers), one has it at D = 256.
 struct Bounds {
     int slots;                            // workgroups resident at a time
     int max_prefix_parts, max_own_parts;  // parts of one row's sum
@@ -177,6 +178,7 @@ int fa_cache_write(const uint16_t* dK, const uint16_t* dV, int64_t k_tok, int64_
     if (int rc = check_cache(cache)) return rc;
     if (tokens < 0 || (int64_t)tokens * cache->heads > 0x7fffffffLL)
         return fail(FA_ERR_SHAPE, "fa_cache_write: tokens must not be negative, tokens * heads below 2^31");
+    if (elapsed_ms) *elapsed_ms = 0.0f;
     if (tokens == 0) return FA_OK;
     if (!dK || !dV || !slots) return fail(FA_ERR_POINTER, "fa_cache_write: null pointer");
     if (!aligned16({dK, dV}) || !whole_pieces({k_tok, k_head, v_tok, v_head}))
@@ -193,9 +195,8 @@ int fa_cache_write(const uint16_t* dK, const uint16_t* dV, int64_t k_tok, int64_
 }
 
 size_t fa_shared_prefix_workspace(int T, int B, int Hq, int Hkv, int D, int prefix_len, int max_k_len) {
-    if (T <= 0 || B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || prefix_len < 0 || prefix_len > kMaxKeys || max_k_len < 0 ||
-        max_k_len > kMaxKeys)
-        return 0;
+    fa_host::clear_error();
+    if (T == 0 || B == 0 || (D != 64 && D != 128 && D != 256) || check_shared(T, B, Hq, Hkv, prefix_len, max_k_len) != FA_OK) return 0;
     return workspace_of(bounds_of(T, B, Hkv, Hq / Hkv, D, prefix_len, max_k_len, fa_host::device_cus()), T, Hq, D);
 }
 
@@ -214,6 +215,7 @@ int fa_forward_shared_prefix(const uint16_t* dQ, int64_t q_tok, int64_t q_head, 
     if (int rc = check_shared(T, B, Hq, Hkv, prefix_len, max_k_len)) return rc;
     if (table_width < 0 || ((int64_t)table_width << log2_page) > kMaxKeys || table_stride < table_width)
         return fail(FA_ERR_SHAPE, "fa_forward_shared_prefix: the block table's rows must name at most 2^30 keys and fit their stride");
+    if (elapsed_ms) *elapsed_ms = 0.0f;
     if (T == 0 || B == 0) return FA_OK;
     if (!dQ || !dO || !q_start || !k_len || (prefix_len > 0 && !prefix_table) || (table_width > 0 && !block_table))
         return fail(FA_ERR_POINTER, "fa_forward_shared_prefix: null pointer");

@@ -118,6 +118,10 @@ def test_workspace_of_refused_sizes_is_none(fa):
     assert L.fa_shared_prefix_workspace(1, 1, 4, 3, 64, 0, 16) == 0
     assert L.fa_shared_prefix_workspace(0, 1, 4, 2, 64, 0, 16) == 0
     assert L.fa_shared_prefix_workspace(1, 1, 4, 2, 64, -1, 16) == 0
+    assert L.fa_shared_prefix_workspace(1, 4001, 4, 2, 64, 0, 16) == 0
+    assert L.fa_shared_prefix_workspace(1, 1, 129, 1, 64, 0, 16) == 0
+    assert L.fa_shared_prefix_workspace(1, 1, 4, 2, 96, 0, 16) == 0
+    assert L.fa_shared_prefix_workspace(1, 1, 4, 2, 64, 0, 16) >= 4 * (64 + 2) * 4
 
 
 def test_python_refusals(fa):

@@ -173,6 +173,44 @@ def test_drawn_shapes(fa, seed):
                     rng.choice([F16, BF16]), rng.choice(["hnd", "nhd", "pool"]), seed=seed), rng.random() < 0.7)
 
 
+@pytest.mark.parametrize("D,dtype", [(64, F16), (64, BF16), (128, F16), (128, BF16), (256, F16), (256, BF16)])
+@pytest.mark.parametrize("rows", [15, 16, 17, 31, 32, 33, 48, 63, 64, 65, 127, 128, 129, 257])
+def test_row_counts(fa, rows, D, dtype):
+    """Around the sizes where the kernel's forms change: one request's rows, and as many single tokens stacked up."""
+    check(fa, Batch(fa, [rows], [rows + 21], 83, 1, 1, D, 16, dtype, seed=rows))
+    check(fa, Batch(fa, [1] * rows, [1 + i % 5 for i in range(rows)], 150, 1, 1, D, 16, dtype, seed=rows + 1))
+
+
+def test_many_requests(fa):
+    """More than one round of 64 and of 128 lengths; idle requests and long ones among them."""
+    rng = random.Random(4)
+    new = [rng.choice([0, 1, 1, 1, 2]) for _ in range(700)]
+    new[77], new[300], new[699] = 140, 33, 200
+    check(fa, Batch(fa, new, [n + rng.randint(0, 40) for n in new], 90, 2, 1, 64, 16, BF16, seed=20))
+    new = [1] * 4000
+    b = Batch(fa, new, [1 + i % 3 for i in range(4000)], 20, 1, 1, 64, 16, F16, seed=21)
+    got = b.call(fa)
+    some = [0, 1, 63, 64, 127, 128, 1999, 3998, 3999]
+    b.new, b.held, b.table = [1] * len(some), [b.held[i] for i in some], [b.table[i] for i in some]
+    b.q, b.start = b.q[some], list(range(len(some) + 1))
+    want, tol = b.expected()
+    assert bool(((got[some].double() - want).abs() <= tol).all())
+    with pytest.raises(fa.FlashAttentionError):
+        Batch(fa, [0] * 4001, [1] * 4001, 0, 1, 1, 64, 16, F16, pad=1).call(fa)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_long_ranges(fa, D):
+    """Keys of one request, and a prefix, over many parts and many runs of 64 page entries, some of which name no page."""
+    check(fa, Batch(fa, [1], [40001], 0, 2, 1, D, 16, F16, seed=22))
+    check(fa, Batch(fa, [3], [20000], 30011, 8, 1, D, 32, BF16, seed=23))
+    b = Batch(fa, [1, 140], [3000, 5000], 9000, 2, 1, D, 16, F16, seed=24)
+    for t in (b.prefix, b.table[0], b.table[1]):
+        for i in range(3, len(t), 71):
+            t[i] = -1
+    check(fa, b)
+
+
 @pytest.mark.parametrize("dtype", [F16, BF16])
 def test_large_scores_and_other_scales(fa, dtype):
     b = Batch(fa, [1, 20, 3], [50, 70, 3], 300, 8, 2, 128, 16, dtype, seed=5, scale=1.7)
