@@ -87,7 +87,8 @@ Bounds bounds_of(int T, int B, int Hkv, int g, int D, int prefix_len, int max_k_
     const int64_t rows = (int64_t)T * g;
     Bounds d;
     d.slots = cus * (D == 256 ? 1 : 2);
-    // enough parts to fill the chip twice over from the prefix alone, or from a few requests' own keys; none shorter than 128 keys
+    // enough parts to fill the chip twice over from the prefix alone, or from a few requests' own keys.  (A part has about 256 keys
+    // at least, so 128 keys a part bound their number, a part that is up to half shorter included.)
     d.max_prefix_parts = prefix_len > 0 ? within(up(2 * d.slots, up(rows, 128) * Hkv), 1, within(up(prefix_len, 128), 1, kMaxParts)) : 0;
     d.max_own_parts = within(up(2 * d.slots, (int64_t)B * Hkv), 4, kMaxParts);
     d.max_own_parts = within(up(max_k_len, 128), 1, d.max_own_parts);
@@ -176,8 +177,8 @@ int fa_cache_write(const uint16_t* dK, const uint16_t* dV, int64_t k_tok, int64_
                    const fa_paged_cache* cache, const int* slots, int tokens, void* stream_, float* elapsed_ms) {
     fa_host::clear_error();
     if (int rc = check_cache(cache)) return rc;
-    if (tokens < 0 || (int64_t)tokens * cache->heads > 0x7fffffffLL)
-        return fail(FA_ERR_SHAPE, "fa_cache_write: tokens must not be negative, tokens * heads below 2^31");
+    if (tokens < 0 || (int64_t)tokens * cache->heads * (cache->head_dim / 8) > 0xffffff00LL)  // (threads of a launch: 32 bits)
+        return fail(FA_ERR_SHAPE, "fa_cache_write: tokens must not be negative, tokens * heads * head_dim below 2^35");
     if (elapsed_ms) *elapsed_ms = 0.0f;
     if (tokens == 0) return FA_OK;
     if (!dK || !dV || !slots) return fail(FA_ERR_POINTER, "fa_cache_write: null pointer");
@@ -221,6 +222,7 @@ int fa_forward_shared_prefix(const uint16_t* dQ, int64_t q_tok, int64_t q_head, 
         return fail(FA_ERR_POINTER, "fa_forward_shared_prefix: null pointer");
     if (!aligned16({dQ, dO}) || !whole_pieces({q_tok, q_head, o_tok, o_head}))
         return fail(FA_ERR_SHAPE, "fa_forward_shared_prefix: q and o must be 16-byte aligned, strides multiples of 8 elements");
+    if (dO == dQ) return fail(FA_ERR_POINTER, "fa_forward_shared_prefix: o must not be q");
     const Bounds d = bounds_of(T, B, Hkv, Hq / Hkv, D, prefix_len, max_k_len, fa_host::device_cus());
     const size_t need = workspace_of(d, T, Hq, D);
     if (need > workspace_bytes || !workspace || !aligned16({workspace})) {

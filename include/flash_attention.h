@@ -277,7 +277,8 @@ const char* fa_kernel_name_block_general(int lq, int lk, int D, int flags, int q
 /* Keys and values in pages of page_size keys (a power of two from 16 to 65536): element (page, head, row, d) of K is
  * k[page * k_strides[0] + head * k_strides[1] + row * k_strides[2] + d], V alike.  16-bit elements, D contiguous;
  * [n_pages][heads][page_size][D], [n_pages][page_size][heads][D] and K and V in one pool are all a choice of strides
- * (multiples of 8 elements; offsets are 64-bit).  head_dim 64, 128 or 256. */
+ * (multiples of 8 elements, rows head_dim to 2^25 elements apart; offsets are 64-bit).  k and v 16-byte aligned; head_dim 64,
+ * 128 or 256; heads at most 65535. */
 typedef struct fa_paged_cache {
     uint16_t* k;
     uint16_t* v;
@@ -300,14 +301,15 @@ typedef struct fa_paged_cache {
  * its row of the table cannot name them, or when its tokens end behind max_tokens: it keeps its length, takes nothing,
  * and its tokens' slots are -1.  Requests that need no page are never refused for want of pages.
  * k_len, n_new and free_count must not overlap the outputs: a program alternates two sets (the free list and the table
- * are updated in place).  B from 1 to 5120; one launch, nothing allocated, no synchronisation. */
+ * are updated in place), nor the outputs each other.  What n_new or an entry of k_len asks beyond these limits is refused or
+ * clamped, never written elsewhere.  B from 1 to 5120, B * table_width below 2^30; one launch, nothing allocated, no synchronisation. */
 int fa_cache_plan(const int* k_len, const int* n_new, int* block_table, int64_t table_stride, int* free_pages,
                   const int* free_count, int* q_start, int* k_len_out, int* slots, int* counts, int B, int table_width,
                   int page_size, int free_cap, int max_tokens, void* stream, float* elapsed_ms);
 
 /* Stores new keys and values: row (t, h) of dK (element t * k_tok + h * k_head + d, strides multiples of 8) and of dV
  * goes into slot slots[t] of the cache.  A slot that is negative or on a page the cache does not have is skipped.  Two
- * tokens with one slot leave either's 16-byte pieces there. */
+ * tokens with one slot leave either's 16-byte pieces there.  dK and dV 16-byte aligned, apart from the cache's rows. */
 int fa_cache_write(const uint16_t* dK, const uint16_t* dV, int64_t k_tok, int64_t k_head, int64_t v_tok, int64_t v_head,
                    const fa_paged_cache* cache, const int* slots, int tokens, void* stream, float* elapsed_ms);
 
@@ -318,13 +320,16 @@ enum { FA_DTYPE_FP16 = 0, FA_DTYPE_BF16 = 1 };
  *            share a K/V head, 16-bit elements of `dtype` (that of the cache)
  * and see the prefix_len keys on the pages prefix_table names, which all requests share, and the k_len[b] keys on the
  * pages of row b of the block table (the new tokens' own among them, the last ones): with FA_FLAG_CAUSAL new token i
- * of n sees keys j <= k_len[b] - n + i of those.  Scores are scaled by `scale` (positive; 1/sqrt(D) as a rule).  prefix_len = 0 is plain paged attention.
- * The prefix is read once for the batch, not once per request.
+ * of n sees keys j <= k_len[b] - n + i of those.  Scores are scaled by `scale` (positive; 1/sqrt(D) as a rule; scaled
+ * scores are taken to stay below 2^26).  prefix_len = 0 is plain paged attention.  The prefix is read once for the batch, not
+ * once per request.
  *   Nothing of a page behind the last key is used, whatever it holds, nor a masked key or value (infinities and NaN
- * among them).  A table entry outside [0, n_pages) names no page: its keys take no part.  Lengths are clamped to what the table
- * names, q_start to [0, T].  Rows that see no key are 0; rows of dO that belong to no request keep their bytes.
- *   B is at most 4000, Hq / cache->heads at most 128.  max_k_len: no request holds more own keys than this as far as the host knows (it bounds the workspace;
- * a longer request is still computed in full).  prefix_len is a host number: a captured launch keeps it.
+ * among them).  A table entry outside [0, n_pages) names no page: its keys take no part.  Lengths are clamped to what the
+ * table names, q_start (ascending) to [0, T].  Rows that see no key are 0; rows of dO that belong to no request keep their
+ * bytes.  dO must not overlap dQ.
+ *   B is at most 4000, Hq / cache->heads at most 128.  max_k_len: no request holds more own keys than this as far as the
+ * host knows (it bounds the workspace; a longer request is still computed in full).  prefix_len is a host number: a captured
+ * launch keeps it.
  *   workspace: fa_shared_prefix_workspace(...) bytes, 16-byte aligned, for this call alone until it has run
  * (FA_ERR_WORKSPACE when it is too small).  Nothing is allocated, nothing waits: the call can be captured. */
 int fa_forward_shared_prefix(const uint16_t* dQ, int64_t q_tok, int64_t q_head, uint16_t* dO, int64_t o_tok, int64_t o_head,

@@ -80,6 +80,23 @@ def test_write_refusals(fa, change, status):
     assert write(fa, cache_struct(fa), **change) == status
 
 
+def test_calls_that_would_not_fit_a_launch(fa):
+    wide = dict(heads=4096, k_strides=(ct.c_int64 * 3)(1 << 22, 64 * 16, 64), v_strides=(ct.c_int64 * 3)(1 << 22, 64 * 16, 64))
+    assert write(fa, cache_struct(fa, **wide), tokens=1 << 17) == 4
+
+
+def test_output_over_the_queries_is_refused(fa):
+    assert shared(fa, cache_struct(fa), o=at(), ws_bytes=1 << 40) == 5
+
+
+def test_calls_without_work_report_no_time(fa):
+    L, ms = fa.lib(), ct.c_float(7.0)
+    assert L.fa_cache_write(None, None, 64, 64, 64, 64, ct.byref(cache_struct(fa)), None, 0, None, ct.byref(ms)) == 0 and ms.value == 0.0
+    ms = ct.c_float(7.0)
+    assert L.fa_forward_shared_prefix(None, 64, 64, None, 64, 64, ct.byref(cache_struct(fa)), None, 0, None, 0, 0, None, None, 0, 1, 4, 0, 1,
+                                      0.125, 0, None, 0, None, ct.byref(ms)) == 0 and ms.value == 0.0
+
+
 def test_nothing_to_write_is_no_error(fa):
     assert write(fa, cache_struct(fa), tokens=0, k=None, v=None) == 0
 

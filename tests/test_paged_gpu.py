@@ -211,6 +211,33 @@ def test_long_ranges(fa, D):
     check(fa, b)
 
 
+def test_ends_of_the_ranges(fa):
+    """128 query heads on one K/V head, 100 K/V heads, the largest pages."""
+    check(fa, Batch(fa, [1, 2, 0, 1], [1, 70, 5, 300], 200, 128, 1, 128, 16, F16, seed=30))
+    check(fa, Batch(fa, [1, 3], [1, 70], 45, 100, 100, 64, 16, BF16, seed=31))
+    check(fa, Batch(fa, [1, 20], [5000, 33], 66000, 4, 2, 64, 65536, F16, seed=32))
+    check(fa, Batch(fa, [3, 150], [9, 4000], 2000, 2, 1, 256, 4096, BF16, seed=33))
+
+
+def test_calls_at_once(fa):
+    """Two batches of different sizes on two streams, a handle and a stream object, with nothing between the calls."""
+    a = Batch(fa, [1] * 40, [50 * i + 1 for i in range(40)], 6000, 8, 2, 128, 16, F16, seed=34)
+    b = Batch(fa, [200, 1], [900, 3000], 3000, 4, 1, 128, 16, F16, seed=35)
+    want = [x.call(fa) for x in (a, b)]
+    args = [(x.q, x.cache, ints(x.start), ints(x.held), ints(x.table), ints(x.prefix), x.prefix_len) for x in (a, b)]
+    s = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [fa.attention_shared_prefix(*args[i % 2], stream=(s[0], s[1].cuda_stream)[i % 2]) for i in range(8)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want[i % 2]) for i, o in enumerate(got))
+
+
+def test_output_over_the_queries_is_refused(fa):
+    b = Batch(fa, [1], [9], 20, 2, 1, 64, 16, F16, seed=36)
+    with pytest.raises(fa.FlashAttentionError):
+        b.call(fa, out=b.q)
+
+
 @pytest.mark.parametrize("dtype", [F16, BF16])
 def test_large_scores_and_other_scales(fa, dtype):
     b = Batch(fa, [1, 20, 3], [50, 70, 3], 300, 8, 2, 128, 16, dtype, seed=5, scale=1.7)
@@ -580,3 +607,62 @@ def test_a_run_of_steps(fa):
                 assert bool(((out[at:at + n].double() - o).abs() <= tolerance(dtype, o, a, size, D, L, vv)).all()), (i, b)
             at += max(n, 0)
         assert bool((out[at:] == 0).all())
+
+
+def test_a_captured_run_of_steps(fa):
+    """Two steps (the two sets of tables in turn) in one graph: plan, write, attention.  Replayed with other lengths each time it
+    leaves what the same calls leave in a twin of the cache."""
+    torch.manual_seed(5)
+    B, page, width, Hq, Hkv, D, T = 5, 16, 8, 4, 2, 64, 24
+    n_new, rows = [ints([0] * B) for _ in range(2)], [torch.randn(3, T, Hq, D, dtype=F16, device=DEV) for _ in range(2)]
+
+    def state():
+        cache = make_cache(fa, 40, Hkv, page, D, F16, seed=37)
+        table, free = torch.full((B, width), -1, dtype=torch.int32, device=DEV), ints(list(range(4, 40)))
+        plans = [fa.make_cache_plan(B, T, DEV) for _ in range(2)]
+        plans[1].k_len.copy_(ints([0] * B))
+        plans[1].counts.copy_(ints([36, 0]))
+        outs = [torch.zeros(T, Hq, D, dtype=F16, device=DEV) for _ in range(2)]
+        return cache, table, free, plans, outs
+
+    prefix = ints([0, 1, 2, 3])
+
+    def steps(cache, table, free, plans, outs):
+        for i in range(2):
+            held = plans[1 - i]
+            p = fa.cache_plan(held.k_len, n_new[i], table, free, held.counts[:1], page, out=plans[i])
+            q, k, v = rows[i]
+            fa.cache_write(k[:, :Hkv], v[:, :Hkv], cache, p.slots)
+            fa.attention_shared_prefix(q, cache, p.q_start, p.k_len, table, prefix, 60, out=outs[i])
+
+    eager, captured = state(), state()
+    steps(*eager)  # (adds nothing)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        steps(*captured)
+    for new in ([[3, 1, 0, 16, 2], [1, 1, 1, 1, 1]], [[1, -2, 20, 0, 1], [1, 4, 1, -17, 1]], [[-4, 1, 1, 17, 1], [20, 1, 1, 1, 1]], [[0] * 5, [1] * 5]):
+        for i in range(2):
+            n_new[i].copy_(ints(new[i]))
+            rows[i].normal_()
+        for o in eager[4] + captured[4]:
+            o.zero_()
+        graph.replay()
+        steps(*eager)
+        torch.cuda.synchronize()
+        for a, b in zip(eager[3] + [eager[1:3]] + [eager[4]], captured[3] + [captured[1:3]] + [captured[4]]):
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
+        assert torch.equal(eager[0].k, captured[0].k) and torch.equal(eager[0].v, captured[0].v)
+        assert captured[3][1].counts[1].item() == 0 and captured[4][1].any()  # (the first step of the last replay adds no token)
+
+
+def test_plan_and_write_on_another_stream_and_timed(fa):
+    cache, side = make_cache(fa, 8, 2, 16, 64, F16, seed=38), torch.cuda.Stream()
+    k, table, free = torch.randn(20, 2, 64, dtype=F16, device=DEV), torch.full((2, 4), -1, dtype=torch.int32, device=DEV), ints(list(range(8)))
+    held, new, count = ints([0, 0]), ints([17, 3]), ints([8])
+    torch.cuda.synchronize()
+    plan, ms = fa.cache_plan(held, new, table, free, count, 16, 20, stream=side, timed=True)
+    assert ms > 0
+    assert fa.cache_write(k, k, cache, plan.slots, stream=side.cuda_stream, timed=True) > 0
+    side.synchronize()
+    at = plan.slots.long()
+    assert torch.equal(cache.k[at // 16, :, at % 16], k) and torch.equal(cache.v[at // 16, :, at % 16], k) and plan.k_len.tolist() == [17, 3]
