@@ -64,10 +64,11 @@ __device__ __forceinline__ void exclusive_sums(int (&v)[K], int (&total)[K], int
 //   its table row, nor its tokens the slot map) is left as it was, and so is every later one that needs pages once the
 //   list has run out; q_start counts its tokens all the same, their slots are -1.
 // Everything is a running sum over the requests, so every workgroup computes the sums itself (8 B per request, read from
-// the L2) and then fills its share of the outputs: one launch, no
-// workgroup waits for another, and no output is an input of another workgroup: a released page that is taken again in
-// the same step is found in its old owner's row, not on the stack.  Bound by latency: the lengths' load, two rounds of
-// sums, the search of a token's request in LDS, the load of its page.
+// the L2) and then fills its share of the outputs: one launch, no workgroup waits for another, and no output is an input
+// of another workgroup: a released page that is taken again in the same step is found in its old owner's row, not on the
+// stack.  Bound by latency: the lengths' load, two rounds of sums, the search of a token's request in LDS, the load of its
+// page.  Measured: 8 requests 2.9 us on the GPU, 1 000 requests 9.1 us a call (LDS scans by doubling steps, lengths read
+// twice: 18.7), 4 096 requests 14.2 (28.3).
 // (Tokens are summed in two halves of 16 bits: 5120 requests of 2^31 - 1 tokens stay within 31 bits each.)
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void fa_cache_plan_kernel(const CachePlanParams p) {
@@ -196,7 +197,9 @@ struct CacheWriteParams {
     int tokens, heads, log2_page, n_pages, log2_chunks;  // 2^log2_chunks pieces of 16 bytes per row
 };
 
-// Row t of head h of the new keys (blockIdx.y = 0) or values (1) into its slot, 16 bytes per thread.
+// Row t of head h of the new keys (blockIdx.y = 0) or values (1) into its slot, 16 bytes per thread: every byte is read
+// once and written once, neighbouring lanes share a row, so a row of 128 to 512 bytes is whole cache lines.  Bound by memory: 65 536
+// tokens of 8 heads at D = 128 take 86 us, 5.8 TB/s of reads and writes; by the launch below some thousand tokens (3 us).
 __global__ __launch_bounds__(256) void fa_cache_write_kernel(const CacheWriteParams p) {
     const bool val = blockIdx.y != 0;
     const uint16_t* src = val ? p.v : p.k;

@@ -6,9 +6,15 @@
 // matrix product for the whole batch, its rows being the g heads of ALL tokens stacked up against each K/V head, so the
 // prefix is read from memory once per 128 stacked rows instead of once per request; the own part has the rows of one
 // request.  Both parts are divided over ranges of keys until the chip is full.
-// A workgroup has 4 waves of 32 rows and walks its range in tiles of kTk keys (transposed scores S^T = K.Q^T, the score
-// registers rounded to 16 bits as B operand of O^T += V^T.P^T, swizzled LDS tiles: the lane geometry of
-// fa_fwd_general_kernel.hpp).  fa_shared_prefix_merge_kernel joins the parts.
+// Both products are transposed (S^T = K.Q^T; the score registers, rounded to the cache's type, are the B operand of
+// O^T += V^T.P^T), scores, maxima, sums and O are 32-bit.  P is rounded once, as every matrix product's operand must be; its
+// sum l is taken before that.  A workgroup has one of two forms: shared_few_rows (bound by reading K and V) and
+// shared_many_rows (bound by the matrix pipe and one wave's instruction issue), chosen by the number of rows.
+// fa_shared_prefix_merge_kernel joins the parts.
+//
+// Measured (one MI355X, kernels alone; a large copy moves 4.9 TB/s, a large matrix product runs at 1.3 PFLOP/s):
+//   one token of each of 128 requests, 1 024 own keys each, no prefix, 8 K/V heads of 4, D = 128: 4.4 TB/s (D = 256 4.2, D = 64 3.7);
+//   one request's prompt against itself, D = 128: 950 - 1 010 TFLOP/s; against a prefix of many rows D = 256 545 - 590, D = 64 535.
 //
 // Masks.  A tile that holds a masked place for some row of the wave (the end of the range, the causal diagonal, a page that
 // is none) takes the masked form of the step: scores of masked places become -inf whatever K holds there, and V is
@@ -133,11 +139,13 @@ struct SharedCfg<256> {
 // The division of a launch into workgroups, from the requests' lengths; every wave computes it for itself (no barrier: all
 // write the same numbers to LDS, each reads what it has written).
 //   A request with fewer than 128 rows (new tokens x g) is short: its rows are stacked up with those of the other short
-// requests against the prefix (items of kind P: one K/V head, 128 stacked rows, a range of the prefix) and alone against
-// its own keys (O: one head, the request's rows, a range of its keys).  A longer request fills row tiles of its own, which walk
-// prefix and own keys in one go (J: one head, 128 of its rows, a range of both): nothing is gained by stacking.
+// requests against the prefix (items of kind P: one K/V head, a row tile of the stack, a range of the prefix) and alone against
+// its own keys (O: one head, a row tile of the request, a range of its keys).  A longer request fills row tiles of its own,
+// which walk prefix and own keys in one go (J: one head, 128 of its rows, a range of both): nothing is gained by stacking.
 //   Ranges take about the same time each, up to half more or less: the launch's key tiles over the workgroups that the chip
-// holds, a tile of many rows counted as kManyCost tiles of few.
+// holds, a tile of many rows counted as kManyCost tiles of few (1 and 3 measured no better), 256 keys at least: a workgroup's
+// start and end cost 13 - 20 thousand cycles, as much as some 500 keys, and each part is written, read and joined again (128:
+// 32 requests behind 8 192 keys 28.7 us, 256: 28.1).
 struct SharedPlan {
     int stacked;        // rows of the short requests, per K/V head
     int prefix_tiles;   // key tiles of the prefix
@@ -309,7 +317,8 @@ __device__ __forceinline__ int64_t part_slot(const SharedPrefixParams& p, const 
 // ---------------------------------------------------------------------------------------------------------------------
 // Up to 16 * RB rows: a single token's heads, or a few tokens'.  The work is bound by reading K and V, so each wave
 // takes a quarter of the item's keys for itself, 16 keys (a granule, on one page) at a time, through a ring of its own:
-// no barrier in the loop, and two granules and more per wave on their way.  S^T = K.Q^T is one 16 x 16 block per 16 rows
+// no barrier in the loop, and two granules and more per wave on their way (K and V through one ring of four waves with a barrier a
+// tile: 3.1 TB/s where this reaches 4.4; D = 256 1.4 and 4.2).  S^T = K.Q^T is one 16 x 16 block per 16 rows
 // (v_mfma 16x16x32), whose registers are the B operand of O^T += V^T.P^T (16x16x16) as they are.  The four waves' sums are joined
 // through LDS at the end.
 // Bank conflicts: a K read takes 16 rows' 16 bytes of one column, a V read 8 rows' 32 bytes (half a wave at a time); the
@@ -586,7 +595,13 @@ __device__ __forceinline__ void shared_few_rows(const SharedPrefixParams& p, con
     }
 }
 
-// Many rows: four waves of 32, key tiles shared through the ring.
+// Many rows: four waves of 32, key tiles of kTk keys shared through a ring of four stages (three on their way), one barrier a
+// tile.  Scores of tile t + 1 run on the matrix pipe beside the exponentials of tile t, then V^T.P^T beside the maximum of t + 1,
+// written out instruction by instruction; O lies in named accumulator registers, which the compiler neither copies nor
+// counts.  That interleaving took one prompt against itself from 760 to 913 TFLOP/s, less scalar work to 954, transfers in pairs
+// and Q's loads beside the first pages' to 1 006.  Bound by one wave's issue: 4.7 cycles an instruction, 8.7 an exponential,
+// beside 32 cycles of matrix work each.  64 rows to a wave would halve the LDS reads and the transfers; built, it ran at 940
+// (two waves to a workgroup) and needed more registers than there are where its other costs were cut.
 template <typename E, int D>
 __device__ __forceinline__ void shared_many_rows(const SharedPrefixParams& p, const SharedItem& it, int tok, char* ring) {
     using HD = HeadDim<D>;
@@ -1041,7 +1056,8 @@ FA_SHARED_KERNEL(fa_shared_prefix_bf16_d256_kernel, __bf16, 256, 256)
 #undef FA_SHARED_KERNEL
 
 // O = sum_s w_s o_s / sum_s w_s l_s,  w_s = exp2(m_s - max_s m_s): D / 4 lanes per row, four parts in flight.  Rows of no
-// request and rows that are written already are left alone.
+// request and rows that are written already are left alone.  Bound by latency and by the bytes of the parts (a row of D floats
+// each, out of the last-level cache as a rule): four parts at a time; 32 requests of 32 heads at D = 128 5.6 us, 128 of 64 heads 8.1.
 template <typename E, int D>
 __global__ __launch_bounds__(256) void fa_shared_prefix_merge_kernel(const SharedPrefixParams p) {
     constexpr int LPR = D / 4, RPB = 256 / LPR, U = 4;
