@@ -92,6 +92,11 @@ Bounds bounds_of(int T, int B, int Hkv, int g, int D, int prefix_len, int max_k_
     d.max_prefix_parts = prefix_len > 0 ? within(up(2 * d.slots, up(rows, 128) * Hkv), 1, within(up(prefix_len, 128), 1, kMaxParts)) : 0;
     d.max_own_parts = within(up(2 * d.slots, (int64_t)B * Hkv), 4, kMaxParts);
     d.max_own_parts = within(up(max_k_len, 128), 1, d.max_own_parts);
+    // Every part is room for all rows.  With many rows few requests can want many parts (the launch's work is divided over the
+    // workgroups), so 1 GiB bounds them, two parts at least; only a request of few rows and a long context beside very many
+    // other rows would take more.
+    const int64_t per_part = rows * Hkv * (D + 2) * (int64_t)sizeof(float);
+    d.max_own_parts = std::min(d.max_own_parts, within((1 << 30) / per_part - d.max_prefix_parts, 2, kMaxParts));
     // (a batch or a request of few rows has two tiles at most, where 128 rows would be one)
     const int64_t p_tiles = prefix_len > 0 ? fa::row_tiles(rows) + 1 : 0, r_tiles = fa::request_tiles_bound(rows, B) + B;
     d.blocks = std::min(Hkv * (p_tiles * d.max_prefix_parts + r_tiles * d.parts()), fa::blocks_bound(p_tiles, r_tiles, Hkv, d.slots));

@@ -141,6 +141,14 @@ def test_workspace_of_refused_sizes_is_none(fa):
     assert L.fa_shared_prefix_workspace(1, 1, 4, 2, 64, 0, 16) >= 4 * (64 + 2) * 4
 
 
+def test_workspace_of_many_rows_is_bounded(fa):
+    """1 GiB, or three parts (a prefix' and two of a request's own keys) and a count a row."""
+    for T, B, Hq, Hkv, D, prefix in [(65536, 1, 64, 8, 128, 0), (4096, 1, 32, 8, 128, 8192), (8000, 8, 32, 8, 128, 8192), (20000, 2, 32, 4, 64, 0),
+                                     (100000, 4, 16, 2, 256, 100), (1, 1, 128, 1, 256, 1 << 20), (512, 512, 64, 8, 128, 1 << 20)]:
+        rows = T * Hq
+        assert fa.lib().fa_shared_prefix_workspace(T, B, Hq, Hkv, D, prefix, 1 << 20) <= max(1 << 30, 3 * rows * (D + 2) * 4) + 4 * rows
+
+
 def test_python_refusals(fa):
     import torch
 

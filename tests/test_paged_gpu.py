@@ -219,6 +219,11 @@ def test_ends_of_the_ranges(fa):
     check(fa, Batch(fa, [3, 150], [9, 4000], 2000, 2, 1, 256, 4096, BF16, seed=33))
 
 
+def test_long_context_beside_very_many_rows(fa):
+    """The workspace of many rows has room for few parts: the one token's 40 001 keys still count, each once."""
+    check(fa, Batch(fa, [1, 19999], [40001, 50], 0, 32, 4, 64, 16, F16, seed=39), causal=False)
+
+
 def test_calls_at_once(fa):
     """Two batches of different sizes on two streams, a handle and a stream object, with nothing between the calls."""
     a = Batch(fa, [1] * 40, [50 * i + 1 for i in range(40)], 6000, 8, 2, 128, 16, F16, seed=34)
