@@ -430,7 +430,9 @@ class PagedCache:
             raise ValueError("k and v must share shape, dtype and device")
         self.k, self.v, self.dtype, self.device, self.device_index = k, v, k.dtype, k.device, k.device.index
         self.n_pages, self.heads, self.page_size, self.head_dim = k.shape
-        self.c = _PagedCacheStruct(k.data_ptr(), v.data_ptr(), (ct.c_int64 * 3)(*k.stride()[:3]), (ct.c_int64 * 3)(*v.stride()[:3]),
+        # (an axis of one may have any stride, also one that the library would refuse)
+        ks, vs = ([D if n == 1 else s for n, s in zip(k.shape[:3], t.stride())] for t, D in ((k, k.shape[3]), (v, k.shape[3])))
+        self.c = _PagedCacheStruct(k.data_ptr(), v.data_ptr(), (ct.c_int64 * 3)(*ks), (ct.c_int64 * 3)(*vs),
                                    self.n_pages, self.page_size, self.heads, self.head_dim)
         self.ref = ct.byref(self.c)
         self.dtype_code = 0 if k.dtype == torch.float16 else 1
@@ -531,7 +533,8 @@ def _token_rows(t, name: str, heads, cache: "PagedCache"):
     if len(shape) != 3 or t.dtype is not cache.dtype or t.get_device() != cache.device_index or shape[2] != cache.head_dim or \
             (heads is not None and shape[1] != heads) or (stride[2] != 1 and t.numel()):
         raise ValueError(f"{name} must be [T, heads, {cache.head_dim}] with contiguous rows, of the cache's dtype and GPU")
-    return t.data_ptr(), stride[0], stride[1]
+    D = shape[2]  # (an axis of one may have any stride)
+    return t.data_ptr(), stride[0] if shape[0] > 1 else D, stride[1] if shape[1] > 1 else D
 
 
 def cache_write(k, v, cache: PagedCache, slots, stream=None, timed: bool = False):

@@ -224,6 +224,37 @@ def test_long_context_beside_very_many_rows(fa):
     check(fa, Batch(fa, [1, 19999], [40001, 50], 0, 32, 4, 64, 16, F16, seed=39), causal=False)
 
 
+def test_tables_without_columns_and_empty_calls(fa):
+    b = Batch(fa, [1, 3], [0, 0], 77, 4, 2, 128, 16, BF16, seed=40)
+    want, tol = b.expected()
+    none = torch.empty(2, 0, dtype=torch.int32, device=DEV)
+    for held in ([0, 0], [5, 900]):  # (the table names no page: clamped to no keys)
+        got = fa.attention_shared_prefix(b.q, b.cache, ints(b.start), ints(held), none, ints(b.prefix), 77)
+        assert bool(((got.double() - want).abs() <= tol).all())
+    assert not fa.attention_shared_prefix(b.q, b.cache, ints(b.start), ints([5, 9]), none).any()
+    assert fa.attention_shared_prefix(b.q[:0], b.cache, ints([0, 0, 0]), ints([5, 9]), none, ints(b.prefix), 77).shape == (0, 4, 128)
+    assert not fa.attention_shared_prefix(b.q, b.cache, ints([0]), ints([]), none[:0], ints(b.prefix), 77).any()
+    plan = fa.cache_plan(ints([3]), ints([2]), ints([[1]]), ints([]), ints([0]), 16, 0)  # no room for a token: refused
+    assert plan.k_len.tolist() == [3] and plan.counts.tolist() == [0, 1] and plan.slots.numel() == 0
+
+
+def test_strides_of_axes_of_one(fa):
+    """One token, one head, one page: the stride of such an axis may be anything."""
+    b = Batch(fa, [1], [9], 0, 1, 1, 64, 16, F16, seed=41)
+    want = b.call(fa)
+    b.q = torch.as_strided(b.q, b.q.shape, (3, 5, 1))
+    assert torch.equal(b.call(fa, out=torch.as_strided(torch.zeros(64, dtype=F16, device=DEV), (1, 1, 64), (1, 1, 1))), want)
+    k, v = b.cache.k[:1], b.cache.v[:1]
+    odd = [torch.as_strided(x, x.shape, (7, 3, 64, 1)) for x in (k, v)]
+    b.cache = fa.PagedCache(*odd)
+    b.table = [[0]]
+    want, tol = b.expected()
+    assert bool(((b.call(fa).double() - want).abs() <= tol).all())
+    rows = torch.as_strided(torch.randn(64, dtype=F16, device=DEV), (1, 1, 64), (1, 1, 1))
+    fa.cache_write(rows, rows, b.cache, ints([4]))
+    assert torch.equal(b.cache.k[0, 0, 4], rows[0, 0])
+
+
 def test_calls_at_once(fa):
     """Two batches of different sizes on two streams, a handle and a stream object, with nothing between the calls."""
     a = Batch(fa, [1] * 40, [50 * i + 1 for i in range(40)], 6000, 8, 2, 128, 16, F16, seed=34)
