@@ -37,18 +37,13 @@ FA_HD int slot_of(int page, int row, int log2_page) {
     return page < 0 || s > 0x7fffffffLL ? -1 : (int)s;
 }
 
-// How a launch of shared-prefix attention is divided.  Row tiles of 128 rows walk `tiles` key tiles each, in `parts_for`
-// ranges of about `steps_for` key tiles: all key tiles of the launch (`work`, per K/V head) over the workgroups that the
-// chip holds (`slots`).  With x = tiles / steps a row tile has max(1, floor(x + 1/2)) ranges at most, i.e. fewer than x
-// beyond the first, and all x together are at most `slots`; the stacked rows' ranges may be made as many as `slots` besides.
-// So blocks_bound holds for any lengths (with half of `slots` for the rounding of the sum).
+// How a launch of shared-prefix attention is divided.  Row tiles of 128 rows (few rows: less) walk `tiles` key tiles each, in
+// tiles / steps ranges, rounded, of about `steps_for` key tiles: all key tiles of the launch (`work`, per K/V head) over the
+// workgroups that the chip holds (`slots`).  With x = tiles / steps a row tile has max(1, floor(x + 1/2)) ranges at most,
+// i.e. fewer than x beyond the first, and all x together are at most `slots`; another `slots` and the half are room for the
+// rounding of the sum.  So blocks_bound holds for any lengths.
 constexpr int kRowTile = 128;
 FA_HD int row_tiles(int64_t rows) { return (int)((rows + kRowTile - 1) / kRowTile); }
-FA_HD int parts_for(int tiles, int steps, int most) {
-    int n = (int)(((int64_t)tiles + (steps >> 1)) / steps);
-    if (n > most) n = most;
-    return n < 1 ? 1 : n;
-}
 FA_HD int steps_for(float work, int heads, int slots, int least) {
     const float per = work * (float)heads / (float)slots;
     const int n = (int)(per < 1e9f ? per : 1e9f) + 1;

@@ -181,6 +181,7 @@ __device__ __forceinline__ int quick_div(int a, int b) { return div_by(a, b, __b
 // R / g for the rows of a launch (R g < 2^32: the launcher's check), by the reciprocal 2^32 / g rounded up.
 __device__ __forceinline__ int div_group(const SharedPrefixParams& p, int R) { return p.g == 1 ? R : (int)__umulhi((unsigned)R, p.g_reciprocal); }
 
+// Ranges of a row tile's `tiles` key tiles: tiles / steps, rounded, from 1 to `most`.
 __device__ __forceinline__ int quick_parts(int tiles, int steps, int most) { return max(1, min(quick_div(tiles + (steps >> 1), steps), most)); }
 
 // Up to few_rows rows are taken few_tile at a time (each tile reads the keys again, from the L2: cheaper than the form for

@@ -15,6 +15,11 @@ static void need(bool ok, const char* what, long a = 0, long b = 0, long c = 0) 
     std::exit(1);
 }
 
+// tiles / steps, rounded, from 1 to `most`: what the kernels do by reciprocals (div_by, checked below)
+static int parts_for(int tiles, int steps, int most) {
+    return std::max(1L, std::min(((long)tiles + steps / 2) / steps, (long)most));
+}
+
 int main() {
     using namespace fa;
     // table entries: inside [0, n_pages) or no page at all
