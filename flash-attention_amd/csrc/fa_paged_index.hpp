@@ -31,6 +31,29 @@ FA_HD int64_t cache_offset(const CacheStrides& s, int page, int head, int row) {
 FA_HD int clamp_int(int x, int lo, int hi) { return x < lo ? lo : x > hi ? hi : x; }
 FA_HD int pages_for(int64_t keys, int log2_page) { return (int)((keys + (1 << log2_page) - 1) >> log2_page); }
 
+// The page that holds keys key .. key + 15 of a walk over `keys` keys (key a multiple of 16), -1 where the table's entry names
+// none.  Keys behind the last one are hidden by the rows' limits whatever is read in their place: they are read from page 0, and
+// what the table holds there, or whether it goes on, does not matter.  (`keys` is at most what the table names.)
+FA_HD int page_of_keys(const int* table, int key, int keys, int log2_page, int n_pages) {
+    if (key >= keys) return 0;
+    const int page = table[key >> log2_page];
+    return page_ok(page, n_pages) ? page : -1;
+}
+// Which 16-key groups lie on no page (bit i: group from + i), of the run of 64 that the transfers have reached and of the one
+// before it: the computation is less than a run behind them.
+struct PagelessGroups {
+    uint64_t before = 0, run = 0;
+    int from = 0;
+    FA_HD void next_run(int first, uint64_t pageless) {
+        before = run;
+        run = pageless;
+        from = first;
+    }
+    FA_HD bool any() const { return (before | run) != 0; }
+    // of the `count` groups from `group` on (count divides 64 and group)
+    FA_HD unsigned of(int group, int count) const { return (unsigned)((group >= from ? run : before) >> (group & 63)) & ((1u << count) - 1); }
+};
+
 // Slot of a key in page `page`: -1 where the page is none or the number passes 31 bits.
 FA_HD int slot_of(int page, int row, int log2_page) {
     const int64_t s = ((int64_t)page << log2_page) + row;

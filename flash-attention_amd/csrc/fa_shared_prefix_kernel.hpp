@@ -299,15 +299,13 @@ struct SharedItem {
     const int* own_table;
 };
 
-// Page of the 16-key group `group` of an item's range, -1 where there is none.
+// Page of the 16-key group `group` of an item's range (page_of_keys; 0 from the range's end on).
 template <int TK>
 __device__ __forceinline__ int page_of_group(const SharedPrefixParams& p, const SharedItem& it, int group, int end) {
     constexpr int CPT = TK / 16;
-    const int u = it.u0 + group / CPT, own = u - it.prefix_tiles;
-    const int* table = own < 0 ? p.prefix_table : it.own_table;
-    const int j = ((own < 0 ? u : own) * TK + 16 * (group % CPT)) >> p.log2_page;
-    const int page = group < end && j < (own < 0 ? pages_for(p.prefix_len, p.log2_page) : p.table_width) ? table[j] : -1;
-    return page_ok(page, p.n_pages) ? page : -1;
+    const int u = it.u0 + group / CPT, own = u - it.prefix_tiles, key = (own < 0 ? u : own) * TK + 16 * (group % CPT);
+    const int keys = group >= end ? 0 : own < 0 ? p.prefix_len : it.own_keys;
+    return page_of_keys(own < 0 ? p.prefix_table : it.own_table, key, keys, p.log2_page, p.n_pages);
 }
 
 // Where a row of the item lies in the workspace, once its sum of parts is known.
@@ -639,7 +637,11 @@ __device__ __forceinline__ void shared_many_rows(const SharedPrefixParams& p, co
     const char* v_head = reinterpret_cast<const char*>(p.vc + head * p.vs.head) + (RPW * wave % 16) * (int64_t)vr;
     const int n_groups = n_tiles * CPT;
     auto load_pages = [&](int group) -> int { return page_of_group<TK>(p, it, group + lane, n_groups); };
-    int pages_next = load_pages(0), any_bad = 0;  // (a tile of an item with a group on no page takes the masked form)
+    int pages_next = load_pages(0);
+    // Tiles of a run of 64 groups some of which lie on no page take the masked form, and those of the run before and behind it: one
+    // number for the steps to look at.
+    PagelessGroups pageless;
+    int near_pageless = 0, had_pageless = 0;
     // (Q's loads go out beside the first pages')
     v8 qf[HD::kSteps];
     {
@@ -652,7 +654,9 @@ __device__ __forceinline__ void shared_many_rows(const SharedPrefixParams& p, co
     auto refill = [&](int g0) {
         const int page = max(pages_next, 0), u = u0 + (g0 + lane) / CPT;
         const int row = ((u < it.prefix_tiles ? u : u - it.prefix_tiles) * TK + 16 * (lane % CPT)) & P1;
-        any_bad |= __builtin_amdgcn_readfirstlane((int)__any(pages_next < 0 && g0 + lane < n_groups));
+        pageless.next_run(g0, __ballot(pages_next < 0 && g0 + lane < n_groups));
+        near_pageless = __builtin_amdgcn_readfirstlane((int)pageless.any());
+        had_pageless |= near_pageless;
         k_at = 2 * ((int64_t)page * p.ks.page + (int64_t)row * p.ks.row);
         v_at = 2 * ((int64_t)page * p.vs.page + (int64_t)row * p.vs.row);
         if (g0 + 64 < n_groups) pages_next = load_pages(g0 + 64);
@@ -718,16 +722,8 @@ __device__ __forceinline__ void shared_many_rows(const SharedPrefixParams& p, co
         own_from = it.prefix_tiles - u0 + (__builtin_amdgcn_readfirstlane(low) + 1) / TK;
     }
     const int cut = p.prefix_len % TK != 0 ? it.prefix_tiles - 1 - u0 : -1;
-    auto needs_mask = [&](int t) -> int { return (int)(t >= own_from) | (int)(t == cut) | any_bad; };
-    auto groups_of = [&](int t) -> unsigned {  // the tile's 16-key groups that lie on a page
-        unsigned g = (1u << CPT) - 1;
-        if (any_bad) {
-#pragma unroll 1
-            for (int c = 0; c < CPT; ++c)
-                if (__builtin_amdgcn_readfirstlane(page_of_group<TK>(p, it, t * CPT + c, n_groups)) < 0) g &= ~(1u << c);
-        }
-        return g;
-    };
+    auto needs_mask = [&](int t) -> int { return (int)(t >= own_from) | (int)(t == cut) | near_pageless; };
+    auto groups_of = [&](int t) -> unsigned { return ((1u << CPT) - 1) & ~pageless.of(t * CPT, CPT); };  // the tile's groups that lie on a page
     auto mask_scores = [&](f32x16 (&s)[KB], int lim, unsigned groups) {
 #pragma unroll
         for (int b = 0; b < KB; ++b)
@@ -893,8 +889,12 @@ __device__ __forceinline__ void shared_many_rows(const SharedPrefixParams& p, co
 #pragma unroll 1
         for (int t = 0; t < n_tiles; ++t) {
             const int u = u0 + t, key = (u < it.prefix_tiles ? u : u - it.prefix_tiles) * TK, lim = limit_of(t);
-            if (!needs_mask(t)) continue;
-            const unsigned groups = groups_of(t);
+            if (!(needs_mask(t) | had_pageless)) continue;
+            unsigned groups = (1u << CPT) - 1;
+            if (had_pageless)
+#pragma unroll 1
+                for (int g = 0; g < CPT; ++g)
+                    if (__builtin_amdgcn_readfirstlane(page_of_group<TK>(p, it, t * CPT + g, n_groups)) < 0) groups &= ~(1u << g);
             const char* v_rows = reinterpret_cast<const char*>(p.vc + head * p.vs.head);
 #pragma unroll 1
             for (int j = 0; j < kTile / 1024; ++j) {
