@@ -164,6 +164,13 @@ struct SharedTables {
     }
 };
 
+// From here on a lane reads what other lanes of its wave wrote to LDS before.  A wave's LDS operations complete in order; this holds
+// the compiler to the order written.
+__device__ __forceinline__ void wave_exchange() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 template <int CTRL, int ROWS>
 __device__ __forceinline__ float dpp_float(float v) {
     return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, true));
@@ -234,6 +241,7 @@ __device__ __forceinline__ int shared_plan(const SharedPrefixParams& p, SharedPl
             tokens += __builtin_amdgcn_readlane(sum, 63);
         }
     }
+    wave_exchange();
     s.stacked = tokens * p.g;
     const int p_tiles = tiles_of(p, s.stacked);
     const bool p_few = s.stacked <= p.few_rows;
@@ -259,6 +267,7 @@ __device__ __forceinline__ int shared_plan(const SharedPrefixParams& p, SharedPl
         if (b < p.B) tab.items[b] = items + sum - n;
         items += __builtin_amdgcn_readlane(sum, 63);
     }
+    wave_exchange();
     return items;
 }
 

@@ -1,6 +1,7 @@
 #!/usr/bin/env python3
 """Build-time audit of the kernels whose inline asm owns accumulator registers: fa_fwd_w64_kernel, its masked
 forms (causal, ragged, both) and its key-split form, the fa_fwd_hd_kernel family and the fa_shared_prefix kernels.
+In the latter, also the tables that a wave's lanes exchange through LDS at the start: see audit_exchange.
 
 These kernels name a[..] literally in their instruction strings; the compiler does not know they hold
 live values.  That is only sound while the compiler itself uses no accumulator register and spills
@@ -59,14 +60,36 @@ def main():
             text = open(out).read()
         for kernel in PAGED_KERNELS:
             audit(text, kernel)
+            audit_exchange(text, kernel)
     print("check_owned_regs: ok (no spills, no scratch, no compiler use of accumulator registers)")
 
 
-def audit(text, KERNEL):
+def body_of(text, KERNEL):
     # the whole function body, up to its end label (a kernel with early exits has several s_endpgm)
     m = re.search(r"^" + KERNEL + r":.*?\n\.Lfunc_end\d+:", text, re.S | re.M)
     if not m:
         sys.exit("check_owned_regs: kernel not found in the assembly")
+    return m
+
+
+def audit_exchange(text, KERNEL):
+    """Until the first barrier of the workgroup the lanes of a wave hand one another table entries through LDS: every LDS read
+    there stands behind a wave barrier that stands behind the writes before it."""
+    written = False
+    for line in body_of(text, KERNEL).group(0).split("\n"):
+        code = line.split(";")[0]
+        if re.search(r"\bs_barrier\b", code):
+            return
+        if "wave barrier" in line:
+            written = False
+        elif re.search(r"\bds_write", code):
+            written = True
+        elif written and re.search(r"\bds_read", code):
+            sys.exit("check_owned_regs: FAILED for " + KERNEL + "\n    an LDS read with no wave barrier behind the writes: " + code.strip())
+
+
+def audit(text, KERNEL):
+    m = body_of(text, KERNEL)
     problems = []
     in_asm = False
     for line in m.group(0).split("\n"):
