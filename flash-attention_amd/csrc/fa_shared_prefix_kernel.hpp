@@ -46,12 +46,9 @@ struct SharedPrefixParams {
     int* row_parts;   // [T * Hq]: parts of the row's sum; 0: its output is written already
     int T, B, Hkv, g, log2_page, n_pages, prefix_len, table_width, causal;
     float scale_log2e;
-    int slots, two_per_unit;        // workgroups that the chip holds at a time; whether two share a compute unit
-    int few_rows, few_tile, log2_few_tile;  // up to this many rows take the form for few, so many at a time
-    unsigned g_reciprocal;          // 2^32 / g, rounded up
-    int max_prefix_parts, max_own_parts;
+    DivisionRule rule;
+    unsigned g_reciprocal;  // 2^32 / g, rounded up
 };
-constexpr int kManyCost = 2;
 
 template <typename E>
 struct Elem;
@@ -125,34 +122,19 @@ template <int D>
 struct SharedCfg;
 template <>
 struct SharedCfg<64> {
-    static constexpr int kTk = 64, kStages = 4, kFewBlocks = 2;  // 16 KiB a stage
+    static constexpr int kTk = key_tile(64), kStages = 4, kFewBlocks = 2;  // 16 KiB a stage
 };
 template <>
 struct SharedCfg<128> {
-    static constexpr int kTk = 32, kStages = 4, kFewBlocks = 1;  // 16 KiB
+    static constexpr int kTk = key_tile(128), kStages = 4, kFewBlocks = 1;  // 16 KiB
 };
 template <>
 struct SharedCfg<256> {
-    static constexpr int kTk = 32, kStages = 4, kFewBlocks = 1;  // 32 KiB
+    static constexpr int kTk = key_tile(256), kStages = 4, kFewBlocks = 1;  // 32 KiB
 };
 
-// The division of a launch into workgroups, from the requests' lengths; every wave computes it for itself (no barrier: all
-// write the same numbers to LDS, each reads what it has written).
-//   A request with fewer than 128 rows (new tokens x g) is short: its rows are stacked up with those of the other short
-// requests against the prefix (items of kind P: one K/V head, a row tile of the stack, a range of the prefix) and alone against
-// its own keys (O: one head, a row tile of the request, a range of its keys).  A longer request fills row tiles of its own,
-// which walk prefix and own keys in one go (J: one head, 128 of its rows, a range of both): nothing is gained by stacking.
-//   Ranges take about the same time each, up to half more or less: the launch's key tiles over the workgroups that the chip
-// holds, a tile of many rows counted as kManyCost tiles of few (1 and 3 measured no better), 256 keys at least: a workgroup's
-// start and end cost 13 - 20 thousand cycles, as much as some 500 keys, and each part is written, read and joined again (128:
-// 32 requests behind 8 192 keys 28.7 us, 256: 28.1).
-struct SharedPlan {
-    int stacked;        // rows of the short requests, per K/V head
-    int prefix_tiles;   // key tiles of the prefix
-    int prefix_parts;   // ranges of the prefix that P items walk
-    int p_items;
-    int steps_few, steps_many;  // key tiles of a range
-};
+// The division of a launch into workgroups (SharedPlan), from the requests' lengths; every wave computes it for itself (no
+// barrier: all write the same numbers to LDS, each reads what it has written).
 // LDS, until the first transfer: per request its first token, its own keys, the stacked tokens and the items before it.
 struct SharedTables {
     int *tok0, *keys, *stacked, *items;
@@ -184,34 +166,19 @@ __device__ __forceinline__ float wave_total(float v) {
     v += dpp_float<0x143, 0xc>(v);
     return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
-__device__ __forceinline__ int quick_div(int a, int b) { return div_by(a, b, __builtin_amdgcn_rcpf((float)b)); }
+struct HardwareRcp {
+    __device__ __forceinline__ float operator()(int b) const { return __builtin_amdgcn_rcpf((float)b); }
+};
 // R / g for the rows of a launch (R g < 2^32: the launcher's check), by the reciprocal 2^32 / g rounded up.
 __device__ __forceinline__ int div_group(const SharedPrefixParams& p, int R) { return p.g == 1 ? R : (int)__umulhi((unsigned)R, p.g_reciprocal); }
-
-// Ranges of a row tile's `tiles` key tiles: tiles / steps, rounded, from 1 to `most`.
-__device__ __forceinline__ int quick_parts(int tiles, int steps, int most) { return max(1, min(quick_div(tiles + (steps >> 1), steps), most)); }
-
-// Up to few_rows rows are taken few_tile at a time (each tile reads the keys again, from the L2: cheaper than the form for
-// many rows, in which one wave of four would compute), more 128 at a time.
-__device__ __forceinline__ int tile_rows(const SharedPrefixParams& p, int rows) { return rows <= p.few_rows ? p.few_tile : kRowTile; }
-__device__ __forceinline__ int tiles_of(const SharedPrefixParams& p, int rows) {
-    return rows <= p.few_rows ? (rows + p.few_tile - 1) >> p.log2_few_tile : row_tiles(rows);
-}
-
-template <int TK>
-__device__ __forceinline__ int request_parts(const SharedPrefixParams& p, const SharedPlan& s, int rows, int keys) {
-    const int own = (keys + TK - 1) / TK;
-    return rows >= kRowTile ? quick_parts(s.prefix_tiles + own, s.steps_many, p.max_prefix_parts + p.max_own_parts)
-                            : quick_parts(own, rows <= p.few_rows ? s.steps_few : s.steps_many, p.max_own_parts);
-}
 
 // Returns the number of items.
 template <int TK>
 __device__ __forceinline__ int shared_plan(const SharedPrefixParams& p, SharedPlan& s, const SharedTables& tab) {
     const int lane = threadIdx.x & 63;
-    s.prefix_tiles = (p.prefix_len + TK - 1) / TK;
+    const int prefix_tiles = (p.prefix_len + TK - 1) / TK;
     int tokens = 0;
-    float few = 0.0f, many = 0.0f;  // key tiles of all row tiles, per K/V head
+    LaunchWork work;
     for (int b0 = 0; b0 < p.B; b0 += 128) {
         int q0[2], q1[2], k[2];
 #pragma unroll
@@ -231,53 +198,24 @@ __device__ __forceinline__ int shared_plan(const SharedPrefixParams& p, SharedPl
                 tab.keys[b] = keys;
                 tab.stacked[b] = tokens + sum - stacked;
                 if (b == p.B - 1) tab.tok0[p.B] = tok0 + n;
-                if (rows >= kRowTile)
-                    many += (float)row_tiles(rows) * (float)(own + s.prefix_tiles);
-                else if (rows > p.few_rows)
-                    many += (float)own;
-                else
-                    few += (float)tiles_of(p, rows) * (float)own;
+                work.add_request(p.rule, rows, own, prefix_tiles);
             }
             tokens += __builtin_amdgcn_readlane(sum, 63);
         }
     }
     wave_exchange();
-    s.stacked = tokens * p.g;
-    const int p_tiles = tiles_of(p, s.stacked);
-    const bool p_few = s.stacked <= p.few_rows;
-    few = wave_total(few), many = wave_total(many);
-    const float prefix = (float)p_tiles * (float)s.prefix_tiles;
-    (p_few ? few : many) += prefix;
-    s.steps_few = steps_for(few + (float)kManyCost * many, p.Hkv, p.slots, 256 / TK);
-    s.steps_many = max(256 / TK, (s.steps_few + kManyCost - 1) / kManyCost);
-    s.prefix_parts = 0;
-    if (s.prefix_tiles > 0 && p_tiles > 0) {
-        s.prefix_parts = quick_parts(s.prefix_tiles, p_few ? s.steps_few : s.steps_many, p.max_prefix_parts);
-        // Two workgroups to a unit: with more P items than units some units hold two, which take nearly twice as long, and the
-        // requests' own items, which wait for memory, find no unit to share with one that computes.
-        const int units = p_tiles * p.Hkv, half = p.slots >> 1;
-        if (p.two_per_unit && units * s.prefix_parts > half && units * s.prefix_parts <= p.slots) s.prefix_parts = max(1, quick_div(half, units));
-    }
-    s.p_items = p_tiles * s.prefix_parts * p.Hkv;
+    work.few = wave_total(work.few), work.many = wave_total(work.many);
+    s = shared_plan_of(p.rule, work, tokens * p.g, prefix_tiles, HardwareRcp());
     int items = s.p_items;
     for (int b0 = 0; b0 < p.B; b0 += 64) {
         const int b = b0 + lane, i = min(b, p.B - 1);
         const int rows = max(tab.tok0[i + 1] - tab.tok0[i], 0) * p.g;
-        const int n = b < p.B ? tiles_of(p, rows) * request_parts<TK>(p, s, rows, tab.keys[i]) * p.Hkv : 0, sum = wave_sum_up(n);
+        const int n = b < p.B ? request_items(p.rule, s, rows, (tab.keys[i] + TK - 1) / TK, HardwareRcp()) : 0, sum = wave_sum_up(n);
         if (b < p.B) tab.items[b] = items + sum - n;
         items += __builtin_amdgcn_readlane(sum, 63);
     }
     wave_exchange();
     return items;
-}
-
-// Item x of units x tiles: eight units at a time, tile by tile, so that the row tiles that read the same keys (one unit: a
-// K/V head and a range) follow each other on one XCD (workgroup ids congruent mod 8 share one and its L2).
-__device__ __forceinline__ void unit_and_tile(int x, int units, int tiles, int& unit, int& tile) {
-    const int full = units >> 3, per = 8 * tiles;
-    const int grp = min(quick_div(x, per), full), r = x - grp * per, w = grp < full ? 8 : units & 7;
-    tile = quick_div(r, w);
-    unit = grp * 8 + (r - tile * w);
 }
 
 // The last b with start[b] <= x, 64 candidates at a time (start in LDS, ascending, start[0] <= x; x uniform).
@@ -1006,7 +944,7 @@ __device__ __forceinline__ void shared_prefix_body(const SharedPrefixParams& p) 
         it.own_keys = it.n_tok = 0;
         it.own_table = nullptr;
         if (it.stacked) {
-            it.rows = plan.stacked, it.parts = plan.prefix_parts, tiles = tiles_of(p, plan.stacked);
+            it.rows = plan.stacked, it.parts = plan.prefix_parts, tiles = tiles_of(p.rule, plan.stacked);
         } else {
             const int b = last_at_most(tab.items, p.B, x);
             tok0 = __builtin_amdgcn_readfirstlane(tab.tok0[b]);
@@ -1014,27 +952,25 @@ __device__ __forceinline__ void shared_prefix_body(const SharedPrefixParams& p) 
             it.own_keys = __builtin_amdgcn_readfirstlane(tab.keys[b]);
             first_item = __builtin_amdgcn_readfirstlane(tab.items[b]);
             it.rows = it.n_tok * p.g;
-            tiles = tiles_of(p, it.rows);
-            it.parts = __builtin_amdgcn_readfirstlane(request_parts<TK>(p, plan, it.rows, it.own_keys));
+            tiles = tiles_of(p.rule, it.rows);
+            it.parts = __builtin_amdgcn_readfirstlane(request_parts(p.rule, plan, it.rows, (it.own_keys + TK - 1) / TK, HardwareRcp()));
             it.own_table = p.block_table + b * p.table_stride;
         }
-        unit_and_tile(x - first_item, p.Hkv * it.parts, tiles, unit, tile);
+        unit_and_tile(x - first_item, p.Hkv * it.parts, tiles, unit, tile, HardwareRcp());
         unit = __builtin_amdgcn_readfirstlane(unit), tile = __builtin_amdgcn_readfirstlane(tile);
-        it.head = __builtin_amdgcn_readfirstlane(quick_div(unit, it.parts)), it.part = unit - it.head * it.parts, it.row0 = tile * tile_rows(p, it.rows);
+        it.head = __builtin_amdgcn_readfirstlane(quick_div(unit, it.parts, HardwareRcp())), it.part = unit - it.head * it.parts, it.row0 = tile * tile_rows(p.rule, it.rows);
         // the key tiles of this row tile: no row of it sees further than its last one
-        const int end = min(it.row0 + tile_rows(p, it.rows), it.rows);
+        const int end = min(it.row0 + tile_rows(p.rule, it.rows), it.rows);
         const int see = p.causal ? min(it.own_keys, it.own_keys - it.n_tok + div_group(p, end - 1) + 1) : it.own_keys;
         const int first = it.stacked || it.rows >= kRowTile ? 0 : plan.prefix_tiles;
         const int last = it.stacked ? plan.prefix_tiles : plan.prefix_tiles + (max(see, 0) + TK - 1) / TK;
         it.before = first > 0 ? plan.prefix_parts : 0;  // (parts that P items add in front of this item's)
-        const int each = __builtin_amdgcn_readfirstlane(quick_div(last - first, it.parts)), over = last - first - each * it.parts;
-        it.u0 = first + it.part * each + min(it.part, over);
-        it.n_tiles = each + (it.part < over ? 1 : 0);
+        range_of(first, last, it.part, it.parts, it.u0, it.n_tiles, HardwareRcp());
         // (the same in every lane, though some came through the vector ALU)
         it.parts = __builtin_amdgcn_readfirstlane(it.parts), it.part = __builtin_amdgcn_readfirstlane(it.part);
         it.before = __builtin_amdgcn_readfirstlane(it.before), it.rows = __builtin_amdgcn_readfirstlane(it.rows);
         it.u0 = __builtin_amdgcn_readfirstlane(it.u0), it.n_tiles = __builtin_amdgcn_readfirstlane(it.n_tiles);
-        few = it.rows <= p.few_rows;
+        few = it.rows <= p.rule.few_rows;
         auto token = [&](int off) -> int {
             const int t = div_group(p, min(it.row0 + off, it.rows - 1));
             if (!it.stacked) return tok0 + t;
@@ -1075,7 +1011,7 @@ __global__ __launch_bounds__(256) void fa_shared_prefix_merge_kernel(const Share
     const int64_t rows = (int64_t)p.T * Hq, i = (int64_t)blockIdx.x * RPB + threadIdx.x / LPR;
     if (i >= rows) return;
     const int tok = (int)(i / Hq), hq = (int)(i - (int64_t)tok * Hq);
-    const int first = p.q_start[0], last = p.q_start[p.B], parts = min(p.row_parts[i], p.max_prefix_parts + p.max_own_parts);
+    const int first = p.q_start[0], last = p.q_start[p.B], parts = min(p.row_parts[i], p.rule.max_prefix_parts + p.rule.max_own_parts);
     if (tok < first || tok >= last || parts <= 0) return;
     const f32x2* ml = reinterpret_cast<const f32x2*>(p.part_ml) + i;
     const float* po = p.part_o + i * D + 4 * c;

@@ -69,40 +69,9 @@ int check_cache(const fa_paged_cache* c) {
 }
 fa::CacheStrides strides_of(const int64_t (&s)[3]) { return {s[0], s[1], s[2]}; }
 
-constexpr int kMaxKeys = 1 << 30, kMaxParts = 64, kMaxBatch = 4000, kMaxGroup = 128;
+constexpr int kMaxKeys = 1 << 30, kMaxBatch = 4000, kMaxGroup = 128;
 
-// What the host decides of a launch: the kernel divides the keys itself, from the lengths (SharedPlan), which the host does
-// not know; here are the bounds that the workspace and the grid are made for.  Two workgroups share a compute unit at D = 64 and
-// 128 (64 KiB of LDS, at most 256 registers), one has it at D = 256.
-struct Bounds {
-    int slots;                            // workgroups resident at a time
-    int max_prefix_parts, max_own_parts;  // parts of one row's sum
-    int64_t blocks;                       // items of any lengths
-    int parts() const { return max_prefix_parts + max_own_parts; }
-};
-
-Bounds bounds_of(int T, int B, int Hkv, int g, int D, int prefix_len, int max_k_len, int cus) {
-    auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
-    auto within = [](int64_t x, int64_t lo, int64_t hi) { return (int)(x < lo ? lo : x > hi ? hi : x); };
-    const int64_t rows = (int64_t)T * g;
-    Bounds d;
-    d.slots = cus * (D == 256 ? 1 : 2);
-    // enough parts to fill the chip twice over from the prefix alone, or from a few requests' own keys.  (A part has about 256 keys
-    // at least, so 128 keys a part bound their number, a part that is up to half shorter included.)
-    d.max_prefix_parts = prefix_len > 0 ? within(up(2 * d.slots, up(rows, 128) * Hkv), 1, within(up(prefix_len, 128), 1, kMaxParts)) : 0;
-    d.max_own_parts = within(up(2 * d.slots, (int64_t)B * Hkv), 4, kMaxParts);
-    d.max_own_parts = within(up(max_k_len, 128), 1, d.max_own_parts);
-    // Every part is room for all rows.  With many rows few requests can want many parts (the launch's work is divided over the
-    // workgroups), so 1 GiB bounds them, two parts at least; only a request of few rows and a long context beside very many
-    // other rows would take more.
-    const int64_t per_part = rows * Hkv * (D + 2) * (int64_t)sizeof(float);
-    d.max_own_parts = std::min(d.max_own_parts, within((1 << 30) / per_part - d.max_prefix_parts, 2, kMaxParts));
-    // (a batch or a request of few rows has two tiles at most, where 128 rows would be one)
-    const int64_t p_tiles = prefix_len > 0 ? fa::row_tiles(rows) + 1 : 0, r_tiles = fa::request_tiles_bound(rows, B) + B;
-    d.blocks = std::min(Hkv * (p_tiles * d.max_prefix_parts + r_tiles * d.parts()), fa::blocks_bound(p_tiles, r_tiles, Hkv, d.slots));
-    return d;
-}
-size_t workspace_of(const Bounds& d, int T, int Hq, int D) {
+size_t workspace_of(const fa::LaunchBounds& d, int T, int Hq, int D) {
     return (size_t)T * Hq * ((size_t)d.parts() * (D + 2) * sizeof(float) + sizeof(int));
 }
 
@@ -120,7 +89,7 @@ int check_shared(int T, int B, int Hq, int Hkv, int prefix_len, int max_k_len) {
 }
 
 template <typename E, int D>
-int launch_shared(const fa::SharedPrefixParams& p, const Bounds& d, hipStream_t stream) {
+int launch_shared(const fa::SharedPrefixParams& p, const fa::LaunchBounds& d, hipStream_t stream) {
     if (d.blocks > 0x7fffffffLL) return fail(FA_ERR_SHAPE, "fa_forward_shared_prefix: grid size out of range");
     constexpr bool half = std::is_same<E, _Float16>::value;
     void (*const kernel)(fa::SharedPrefixParams) = D == 64    ? (half ? fa::fa_shared_prefix_f16_d64_kernel : fa::fa_shared_prefix_bf16_d64_kernel)
@@ -203,7 +172,7 @@ int fa_cache_write(const uint16_t* dK, const uint16_t* dV, int64_t k_tok, int64_
 size_t fa_shared_prefix_workspace(int T, int B, int Hq, int Hkv, int D, int prefix_len, int max_k_len) {
     fa_host::clear_error();
     if (T == 0 || B == 0 || (D != 64 && D != 128 && D != 256) || check_shared(T, B, Hq, Hkv, prefix_len, max_k_len) != FA_OK) return 0;
-    return workspace_of(bounds_of(T, B, Hkv, Hq / Hkv, D, prefix_len, max_k_len, fa_host::device_cus()), T, Hq, D);
+    return workspace_of(fa::launch_bounds_of(T, B, Hkv, Hq / Hkv, D, prefix_len, max_k_len, fa_host::device_cus()), T, Hq, D);
 }
 
 int fa_forward_shared_prefix(const uint16_t* dQ, int64_t q_tok, int64_t q_head, uint16_t* dO, int64_t o_tok, int64_t o_head,
@@ -228,7 +197,7 @@ int fa_forward_shared_prefix(const uint16_t* dQ, int64_t q_tok, int64_t q_head, 
     if (!aligned16({dQ, dO}) || !whole_pieces({q_tok, q_head, o_tok, o_head}))
         return fail(FA_ERR_SHAPE, "fa_forward_shared_prefix: q and o must be 16-byte aligned, strides multiples of 8 elements");
     if (dO == dQ) return fail(FA_ERR_POINTER, "fa_forward_shared_prefix: o must not be q");
-    const Bounds d = bounds_of(T, B, Hkv, Hq / Hkv, D, prefix_len, max_k_len, fa_host::device_cus());
+    const fa::LaunchBounds d = fa::launch_bounds_of(T, B, Hkv, Hq / Hkv, D, prefix_len, max_k_len, fa_host::device_cus());
     const size_t need = workspace_of(d, T, Hq, D);
     if (need > workspace_bytes || !workspace || !aligned16({workspace})) {
         char text[160];
@@ -248,9 +217,7 @@ int fa_forward_shared_prefix(const uint16_t* dQ, int64_t q_tok, int64_t q_head, 
     p.T = T, p.B = B, p.Hkv = Hkv, p.g = Hq / Hkv, p.log2_page = log2_page, p.n_pages = cache->n_pages;
     p.prefix_len = prefix_len, p.table_width = table_width, p.causal = flags & FA_FLAG_CAUSAL;
     p.scale_log2e = scale * 1.44269504088896340736f;
-    p.slots = d.slots, p.two_per_unit = D != 256, p.few_tile = D == 64 ? 32 : 16, p.log2_few_tile = D == 64 ? 5 : 4, p.few_rows = 2 * p.few_tile;
-    p.g_reciprocal = fa::group_reciprocal(p.g);
-    p.max_prefix_parts = d.max_prefix_parts, p.max_own_parts = d.max_own_parts;
+    p.rule = d.rule, p.g_reciprocal = fa::group_reciprocal(p.g);
     hipStream_t stream = static_cast<hipStream_t>(stream_);
     return timed(stream, elapsed_ms, [&]() -> int {
         if (dtype == FA_DTYPE_FP16)

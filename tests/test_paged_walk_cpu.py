@@ -10,7 +10,7 @@ from conftest import ROOT
 CPP = os.path.join(ROOT, "tests", "cpp")
 
 
-@pytest.mark.parametrize("program", ["paged_walk_check"])
+@pytest.mark.parametrize("program", ["paged_walk_check", "paged_division_check"])
 def test_host_program(program):
     subprocess.run(["make", "-s", "-C", CPP, program], check=True)
     r = subprocess.run([os.path.join(CPP, program)], capture_output=True, text=True)
