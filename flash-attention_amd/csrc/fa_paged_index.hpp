@@ -189,9 +189,11 @@ FA_HD int64_t request_tiles_bound(int64_t rows, int requests) { return rows / kR
 FA_HD int64_t blocks_bound(int64_t prefix_row_tiles, int64_t request_row_tiles, int heads, int slots) {
     return heads * (prefix_row_tiles + request_row_tiles) + 5 * (int64_t)slots / 2 + 1;
 }
+constexpr int64_t part_bytes(int D) { return (D + 2) * (int64_t)sizeof(float); }  // of one row: O, the maximum and the sum
 struct LaunchBounds {
     DivisionRule rule;
     int64_t blocks;  // items of any lengths
+    int parts_kept;  // parts of every row that the workspace holds
     int parts() const { return rule.max_prefix_parts + rule.max_own_parts; }
 };
 // Two workgroups share a compute unit at D = 64 and 128 (64 KiB of LDS, at most 256 registers), one has it at D = 256.
@@ -210,11 +212,13 @@ inline LaunchBounds launch_bounds_of(int T, int B, int Hkv, int g, int D, int pr
     d.max_own_parts = within(up(2 * d.slots, (int64_t)B * Hkv), 4, kMaxParts);
     d.max_own_parts = within(up(max_k_len, 128), 1, d.max_own_parts);
     // Every part is room for all rows.  With many rows few requests can want many parts (the launch's work is divided over the
-    // workgroups), so 1 GiB bounds them, two parts at least; only a request of few rows and a long context beside very many
-    // other rows would take more.
-    const int64_t per_part = rows * Hkv * (D + 2) * (int64_t)sizeof(float);
-    const int held = within((1 << 30) / per_part - d.max_prefix_parts, 2, kMaxParts);
+    // workgroups, and the row tiles alone fill them several times over), so 1 GiB bounds them, one of own keys at least; only a
+    // request of few rows and a long context beside very many other rows would take more.  A row of one part goes to the output
+    // at once, so a launch whose rows all have one needs no room for it: it is left out where it would pass the bound.
+    const int64_t per_part = rows * Hkv * part_bytes(D), most_bytes = 1 << 30;
+    const int held = within(most_bytes / per_part - d.max_prefix_parts, 1, kMaxParts);
     if (d.max_own_parts > held) d.max_own_parts = held;
+    b.parts_kept = b.parts() == 1 && per_part > most_bytes ? 0 : b.parts();
     // (a batch or a request of few rows has two tiles at most, where 128 rows would be one)
     const int64_t p_tiles = prefix_len > 0 ? row_tiles(rows) + 1 : 0, r_tiles = request_tiles_bound(rows, B) + B;
     const int64_t most = Hkv * (p_tiles * d.max_prefix_parts + r_tiles * b.parts()), sum = blocks_bound(p_tiles, r_tiles, Hkv, d.slots);

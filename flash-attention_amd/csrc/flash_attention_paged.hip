@@ -72,7 +72,7 @@ fa::CacheStrides strides_of(const int64_t (&s)[3]) { return {s[0], s[1], s[2]}; 
 constexpr int kMaxKeys = 1 << 30, kMaxBatch = 4000, kMaxGroup = 128;
 
 size_t workspace_of(const fa::LaunchBounds& d, int T, int Hq, int D) {
-    return (size_t)T * Hq * ((size_t)d.parts() * (D + 2) * sizeof(float) + sizeof(int));
+    return (size_t)T * Hq * ((size_t)d.parts_kept * fa::part_bytes(D) + sizeof(int));
 }
 
 int check_shared(int T, int B, int Hq, int Hkv, int prefix_len, int max_k_len) {
@@ -212,8 +212,8 @@ int fa_forward_shared_prefix(const uint16_t* dQ, int64_t q_tok, int64_t q_head, 
     p.prefix_table = prefix_table, p.block_table = block_table, p.table_stride = table_stride;
     p.q_start = q_start, p.k_len = k_len;
     p.part_o = static_cast<float*>(workspace);
-    p.part_ml = p.part_o + (size_t)d.parts() * T * Hq * D;
-    p.row_parts = reinterpret_cast<int*>(p.part_ml + (size_t)d.parts() * T * Hq * 2);
+    p.part_ml = p.part_o + (size_t)d.parts_kept * T * Hq * D;
+    p.row_parts = reinterpret_cast<int*>(p.part_ml + (size_t)d.parts_kept * T * Hq * 2);
     p.T = T, p.B = B, p.Hkv = Hkv, p.g = Hq / Hkv, p.log2_page = log2_page, p.n_pages = cache->n_pages;
     p.prefix_len = prefix_len, p.table_width = table_width, p.causal = flags & FA_FLAG_CAUSAL;
     p.scale_log2e = scale * 1.44269504088896340736f;

@@ -48,6 +48,9 @@ int main() {
         const DivisionRule& d = bounds.rule;
         const Rcp rcp{std::rand() % 3 - 1};
         need(d.max_prefix_parts <= kMaxParts && d.max_own_parts <= kMaxParts && (d.max_prefix_parts > 0) == (prefix_len > 0) && d.max_own_parts > 0, "parts", trial);
+        const int64_t held = (int64_t)bounds.parts_kept * T * Hkv * g * part_bytes(D);
+        need(held <= 1 << 30 || (bounds.parts_kept == 2 && d.max_prefix_parts == 1), "bytes of the parts", trial, held, bounds.parts_kept);
+        need(bounds.parts_kept == bounds.parts() || (bounds.parts_kept == 0 && bounds.parts() == 1), "parts that are written have room", trial);
         // the kernels' division
         const int prefix_tiles = (prefix_len + TK - 1) / TK;
         auto own_tiles = [&](int b) { return (keys[b] + TK - 1) / TK; };

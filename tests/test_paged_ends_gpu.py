@@ -41,3 +41,12 @@ def test_missing_pages_here_and_there(fa, D):
                     t[i] = -1
         check(fa, b)
         check(fa, b, causal=False)
+
+
+def test_long_contexts_beside_so_many_rows_that_none_is_divided(fa):
+    """22 000 tokens and more of 64 heads: the workspace has one part of own keys, or, without a prefix, none."""
+    check(fa, Batch(fa, [1, 32999], [40001, 50], 0, 64, 4, 64, 16, F16, seed=53), causal=False)
+    check(fa, Batch(fa, [3, 21997], [20000, 60], 500, 64, 4, 64, 16, BF16, seed=54), causal=False)
+    b = Batch(fa, [2, 33000], [30000, 40], 0, 64, 8, 128, 16, BF16, seed=55)
+    assert fa.lib().fa_shared_prefix_workspace(33002, 2, 64, 8, 128, 0, 1 << 20) == 4 * 33002 * 64
+    check(fa, b, causal=False)

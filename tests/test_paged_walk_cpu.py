@@ -34,3 +34,15 @@ def test_lanes_exchange_tables_behind_a_barrier(tmp_path):
     tool.audit_exchange(planted % "; wave barrier\n", "k")
     with pytest.raises(SystemExit):
         tool.audit_exchange(planted % "", "k")
+
+
+def test_workspace_of_long_prompts(fa):
+    """Long prompts' row tiles fill the chip by themselves: their rows are not divided, and no room for parts of them is asked for
+    beyond 1 GiB, or beyond one part behind the prefix and one of the prefix."""
+    for T, B, Hq, Hkv, D in [(65536, 1, 64, 8, 128), (40000, 3, 64, 8, 128), (65536, 4, 32, 8, 256), (200000, 16, 32, 32, 64)]:
+        rows, part = T * Hq, (D + 2) * 4
+        assert rows * part > 1 << 30
+        assert fa.lib().fa_shared_prefix_workspace(T, B, Hq, Hkv, D, 0, 1 << 20) == 4 * rows
+        assert fa.lib().fa_shared_prefix_workspace(T, B, Hq, Hkv, D, 5000, 1 << 20) == rows * (2 * part + 4)
+    rows, part = 33000 * 64, 66 * 4
+    assert fa.lib().fa_shared_prefix_workspace(33000, 2, 64, 4, 64, 0, 1 << 20) == rows * (part + 4)
