@@ -504,7 +504,8 @@ def cache_plan(k_len, n_new, block_table, free_pages, free_count, page_size: int
     """``fa_cache_plan``: block table, slot map and lengths of one serving step, on the GPU.  ``k_len``, ``n_new`` [B] keys
     each request holds and adds (negative: drops from its end); ``block_table`` [B, width] and the stack ``free_pages`` are
     updated in place, ``free_count`` [1] counts its pages.  All int32 GPU tensors.  Returns a ``CachePlan`` (``out``, or a
-    new one for ``max_tokens`` tokens); a refused request keeps its ``k_len``."""
+    new one for ``max_tokens`` tokens); a refused request (``n_new`` > 0) keeps its ``k_len``, and attention's output
+    means nothing on its rows, which ``q_start`` counts."""
     import torch
 
     B, dev = k_len.numel(), k_len.get_device()

@@ -299,7 +299,10 @@ typedef struct fa_paged_cache {
  *   counts[2]      free pages left, requests refused
  * A request is refused when its pages, counted with those of every request before it, are more than there are, when
  * its row of the table cannot name them, or when its tokens end behind max_tokens: it keeps its length, takes nothing,
- * and its tokens' slots are -1.  Requests that need no page are never refused for want of pages.
+ * and its tokens' slots are -1.  Requests that need no page are never refused for want of pages.  The refused ones are those with
+ * n_new[b] > 0 and k_len_out[b] as before.  q_start counts their tokens, so the rows stay where the caller put them; their keys are
+ * not in the cache, and attention takes them for the last keys that the request holds: the outputs of those rows mean nothing,
+ * those of the other requests are not touched by it.
  * k_len, n_new and free_count must not overlap the outputs: a program alternates two sets (the free list and the table
  * are updated in place), nor the outputs each other.  What n_new or an entry of k_len asks beyond these limits is refused or
  * clamped, never written elsewhere.  B from 1 to 5120, B * table_width below 2^30; one launch, nothing allocated, no synchronisation. */

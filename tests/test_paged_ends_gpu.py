@@ -50,3 +50,33 @@ def test_long_contexts_beside_so_many_rows_that_none_is_divided(fa):
     b = Batch(fa, [2, 33000], [30000, 40], 0, 64, 8, 128, 16, BF16, seed=55)
     assert fa.lib().fa_shared_prefix_workspace(33002, 2, 64, 8, 128, 0, 1 << 20) == 4 * 33002 * 64
     check(fa, b, causal=False)
+
+
+def test_refused_requests_in_a_step(fa):
+    """Of five requests the second and the fourth find no page: told apart by their lengths, nothing of them stored, the rows of the
+    others as if they were alone, and their own as if their tokens were the last keys held."""
+    page, Hq, Hkv, D = 16, 4, 2, 64
+    held, new, fits = [16, 30, 5, 32, 3], [10, 20, 11, 1, 1], [True, False, True, False, True]
+    b = Batch(fa, new, [h + n * ok for h, n, ok in zip(held, new, fits)], 50, Hq, Hkv, D, page, BF16, seed=56)
+    owned = [-(-h // page) for h in held]
+    table = ints([t[:n] + [-1] * (4 - n) for t, n in zip(b.table, owned)])
+    free = ints([b.table[0][1]])  # one page, which the first request takes
+    plan = fa.cache_plan(ints(held), ints(new), table, free, ints([1]), page, sum(new))
+    assert plan.counts.tolist() == [0, 2] and plan.q_start.tolist() == b.start
+    grown = (plan.k_len - ints(held)).tolist()
+    assert [g == n for g, n in zip(grown, new)] == fits and plan.k_len.tolist() == b.held
+    stored = [s >= 0 for s in plan.slots.tolist()]
+    assert stored == sum(([ok] * n for ok, n in zip(fits, new)), [])
+    k, v = torch.randn(2, sum(new), Hkv, D, dtype=BF16, device=DEV)
+    before = b.cache.k.clone()
+    fa.cache_write(k, v, b.cache, plan.slots)
+    assert (before != b.cache.k).any(-1).sum() == Hkv * sum(stored)
+    got = fa.attention_shared_prefix(b.q, b.cache, plan.q_start, plan.k_len, table, ints(b.prefix), 50)
+    b.table = table.tolist()
+    want, tol = b.expected()
+    assert bool(((got.double() - want).abs() <= tol).all())
+    keep = torch.tensor(stored, device=DEV)
+    b.new, b.held, b.table = ([x for x, ok in zip(y, fits) if ok] for y in (b.new, b.held, b.table))
+    b.q, b.start = b.q[keep], [0, 10, 21, 22]
+    want, tol = b.expected()
+    assert bool(((got[keep].double() - want).abs() <= tol).all())
