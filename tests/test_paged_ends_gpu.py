@@ -80,3 +80,62 @@ def test_refused_requests_in_a_step(fa):
     b.q, b.start = b.q[keep], [0, 10, 21, 22]
     want, tol = b.expected()
     assert bool(((got[keep].double() - want).abs() <= tol).all())
+
+
+def put(b, pages, key, head, column, value):
+    b.cache.v[pages[key // b.page], head, key % b.page, column] = value
+
+
+@pytest.mark.parametrize("D,dtype", KINDS)
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_specials_in_values_reach_the_rows_that_see_them(fa, D, dtype, bad):
+    """In V alone, in tiles that are masked for some rows of a wave: the rows that see the key have it in its column, all other
+    elements keep their bits.  A prompt's own keys, the cut tile of a prefix that many rows stack up against, a few rows."""
+    # 150 tokens of two heads a K/V head behind a prefix and 75 keys of their own
+    b = Batch(fa, [150], [225], 37, 4, 2, D, 16, dtype, seed=57)
+    clean = check(fa, b)
+    put(b, b.table[0], 75 + 90, 0, 5, bad)
+    put(b, b.table[0], 75 + 120, 0, 5, -bad)
+    put(b, b.table[0], 75 + 149, 1, D - 1, bad)
+    got = b.call(fa)
+    hit = torch.zeros_like(got, dtype=torch.bool)
+    hit[90:, :2, 5] = True
+    hit[149:, 2:, D - 1] = True
+    assert torch.equal(got[~hit], clean[~hit])
+    seen = torch.cat([got[90:120, :2, 5].flatten(), got[149, 2:, D - 1]])
+    assert bool(seen.isnan().all()) if math.isnan(bad) else bool((seen == bad).all())
+    assert bool(got[120:, :2, 5].isnan().all())  # (inf - inf)
+
+    # 140 single tokens; the prefix' last key, and what lies behind it on its last page
+    for count in (140, 12):
+        b = Batch(fa, [1] * count, [1 + i % 40 for i in range(count)], 1000 + 5, 4, 2, D, 16, dtype, seed=58)
+        clean = check(fa, b)
+        put(b, b.prefix, 1004, 1, 7, bad)
+        put(b, b.prefix, 960, 0, 8, bad)
+        put(b, b.prefix, 1005, 0, slice(None), bad)
+        put(b, b.table[3], b.held[3] - 1, 1, 9, bad)
+        got = b.call(fa)
+        hit = torch.zeros_like(got, dtype=torch.bool)
+        hit[:, 2:, 7] = True
+        hit[:, :2, 8] = True
+        hit[3, 2:, 9] = True
+        assert torch.equal(got[~hit], clean[~hit])
+        assert bool(got[hit].isnan().all()) if math.isnan(bad) else bool((got[hit] == bad).all())
+
+
+@pytest.mark.parametrize("D,dtype", KINDS)
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_page_0_is_nothing_where_no_page_is_named(fa, D, dtype, bad):
+    """Page 0, which the kernels read where a table names no page and behind the last key, full of NaN or infinities; nobody's own."""
+    for new, held, prefix in [([1, 9, 2], [100, 90, 40], 200 + 21), ([150, 3], [150 + 471, 40], 1024 + 17), ([1] * 140, [1 + i % 37 for i in range(140)], 517)]:
+        b = Batch(fa, new, held, prefix, 2, 1, D, 16, dtype, seed=59)
+        used = set(b.prefix + sum(b.table, []))
+        spare = min(p for p in range(1, b.cache.n_pages) if p not in used)
+        b.prefix, b.table = [spare if p == 0 else p for p in b.prefix], [[spare if p == 0 else p for p in t] for t in b.table]
+        clean = check(fa, b)
+        b.cache.k[0] = b.cache.v[0] = bad
+        assert torch.equal(b.call(fa), clean)
+        b.prefix[3], b.prefix[7], b.table[1][1] = -1, b.cache.n_pages, -2 ** 31
+        b.table[0][2 % len(b.table[0])] = 2 ** 31 - 1
+        check(fa, b)
+        check(fa, b, causal=False)
