@@ -40,20 +40,13 @@ FA_HD int page_of_keys(const int* table, int key, int keys, int log2_page, int n
     const int page = table[key >> log2_page];
     return page_ok(page, n_pages) ? page : -1;
 }
-// Which 16-key groups lie on no page (bit i: group from + i), of the run of 64 that the transfers have reached and of the one
-// before it: the computation is less than a run behind them.
-struct PagelessGroups {
-    uint64_t before = 0, run = 0;
-    int from = 0;
-    FA_HD void next_run(int first, uint64_t pageless) {
-        before = run;
-        run = pageless;
-        from = first;
-    }
-    FA_HD bool any() const { return (before | run) != 0; }
-    // of the `count` groups from `group` on (count divides 64 and group)
-    FA_HD unsigned of(int group, int count) const { return (unsigned)((group >= from ? run : before) >> (group & 63)) & ((1u << count) - 1); }
-};
+// The kernels read a table 64 groups of 16 keys (a run) at a time, and keep which of a run's groups lie on no page (bit i: group i of
+// the run) for the run that the transfers have reached and for the one before it: the computation is less than a run behind them.
+// Those of the `per` groups (a divisor of 64) of tile `tile`, looked at when tile + ahead is the last tile transferred.
+FA_HD unsigned pageless_groups(uint64_t before, uint64_t run, int tile, int ahead, int per) {
+    const int group = tile * per, reached = ((tile + ahead) * per) & ~63;
+    return (unsigned)((group >= reached ? run : before) >> (group & 63)) & ((1u << per) - 1);
+}
 
 // Slot of a key in page `page`: -1 where the page is none or the number passes 31 bits.
 FA_HD int slot_of(int page, int row, int log2_page) {

@@ -585,10 +585,9 @@ __device__ __forceinline__ void shared_many_rows(const SharedPrefixParams& p, co
     const int n_groups = n_tiles * CPT;
     auto load_pages = [&](int group) -> int { return page_of_group<TK>(p, it, group + lane, n_groups); };
     int pages_next = load_pages(0);
-    // Tiles of a run of 64 groups some of which lie on no page take the masked form, and those of the run before and behind it: one
-    // number for the steps to look at.
-    PagelessGroups pageless;
-    int near_pageless = 0, had_pageless = 0;
+    // Lane L: whether group L of the run of 64 lies on no page (bit 0), of the run before (bit 1), of any run so far (bit 2).  Tiles
+    // near such a group take the masked form, by the one number that the steps look at.
+    int pageless = 0, near_pageless = 0;
     // (Q's loads go out beside the first pages')
     v8 qf[HD::kSteps];
     {
@@ -601,9 +600,8 @@ __device__ __forceinline__ void shared_many_rows(const SharedPrefixParams& p, co
     auto refill = [&](int g0) {
         const int page = max(pages_next, 0), u = u0 + (g0 + lane) / CPT;
         const int row = ((u < it.prefix_tiles ? u : u - it.prefix_tiles) * TK + 16 * (lane % CPT)) & P1;
-        pageless.next_run(g0, __ballot(pages_next < 0 && g0 + lane < n_groups));
-        near_pageless = __builtin_amdgcn_readfirstlane((int)pageless.any());
-        had_pageless |= near_pageless;
+        pageless = (pageless & 4) | (pageless & 1) << 1 | (pages_next < 0 && g0 + lane < n_groups ? 5 : 0);
+        near_pageless = __builtin_amdgcn_readfirstlane((int)__any(pageless & 3));
         k_at = 2 * ((int64_t)page * p.ks.page + (int64_t)row * p.ks.row);
         v_at = 2 * ((int64_t)page * p.vs.page + (int64_t)row * p.vs.row);
         if (g0 + 64 < n_groups) pages_next = load_pages(g0 + 64);
@@ -670,7 +668,10 @@ __device__ __forceinline__ void shared_many_rows(const SharedPrefixParams& p, co
     }
     const int cut = p.prefix_len % TK != 0 ? it.prefix_tiles - 1 - u0 : -1;
     auto needs_mask = [&](int t) -> int { return (int)(t >= own_from) | (int)(t == cut) | near_pageless; };
-    auto groups_of = [&](int t) -> unsigned { return ((1u << CPT) - 1) & ~pageless.of(t * CPT, CPT); };  // the tile's groups that lie on a page
+    // the groups of tile t that lie on a page; looked at when the transfers have reached tile t + ST - 2
+    auto groups_of = [&](int t) -> unsigned {
+        return ((1u << CPT) - 1) & ~pageless_groups(__ballot((pageless & 2) != 0), __ballot((pageless & 1) != 0), t, ST - 2, CPT);
+    };
     auto mask_scores = [&](f32x16 (&s)[KB], int lim, unsigned groups) {
 #pragma unroll
         for (int b = 0; b < KB; ++b)
@@ -831,12 +832,13 @@ __device__ __forceinline__ void shared_many_rows(const SharedPrefixParams& p, co
     if (__builtin_expect(specials != 0, 0)) {
         // the values taken out of masked tiles, to the rows that do see them: those tiles' V once more, in the quarter of the
         // ring that is this wave's own now
+        const int had_pageless = __builtin_amdgcn_readfirstlane((int)__any(pageless & 4));
         char* mine = ring + wave * (ST * kStage / 4);
         const unsigned mine_lds = ring_lds + (unsigned)(wave * (ST * kStage / 4));
 #pragma unroll 1
         for (int t = 0; t < n_tiles; ++t) {
             const int u = u0 + t, key = (u < it.prefix_tiles ? u : u - it.prefix_tiles) * TK, lim = limit_of(t);
-            if (!(needs_mask(t) | had_pageless)) continue;
+            if (!(needs_mask(t) | had_pageless)) continue;  // (the other tiles' were multiplied as they are)
             unsigned groups = (1u << CPT) - 1;
             if (had_pageless)
 #pragma unroll 1

@@ -42,22 +42,20 @@ int main() {
         const int holes = trial % 3 ? std::rand() % 4 : 0;
         for (int i = 0; i < holes; ++i) table[std::rand() % pages_for(keys, 4)] = -1;
         auto pageless_at = [&](int g) { return g < groups && page_of_keys(table.data(), 16 * g, keys, 4, n_pages) < 0; };
-        PagelessGroups acc;
+        uint64_t before = 0, run = 0;
         auto transfer = [&](int t) {
             if (t * per % 64 != 0) return;
-            uint64_t m = 0;
-            for (int i = 0; i < 64; ++i) m |= (uint64_t)pageless_at(t * per + i) << i;
-            acc.next_run(t * per, m);
+            before = run, run = 0;
+            for (int i = 0; i < 64; ++i) run |= (uint64_t)pageless_at(t * per + i) << i;
         };
         auto look = [&](int t) {
             unsigned want = 0;
             for (int i = 0; i < per; ++i) want |= (unsigned)pageless_at(t * per + i) << i;
-            need(acc.of(t * per, per) == want, "groups of a tile", trial, t, want);
-            need(want == 0 || acc.any(), "a tile with a group on no page", trial, t);
-            if (holes == 0) need(!acc.any(), "a prefix' or a request's end is no missing page", trial, t, keys);
+            need(pageless_groups(before, run, t, 2, per) == want, "groups of a tile", trial, t, want);
+            if (holes == 0) need((before | run) == 0, "a prefix' or a request's end is no missing page", trial, t, keys);
             bool near = false;
             for (int g = std::max(0, t * per - 192); g < t * per + 192; ++g) near = near || pageless_at(g);
-            if (!near) need(!acc.any(), "a missing page far away", trial, t);
+            if (!near) need((before | run) == 0, "a missing page far away", trial, t);
         };
         for (int t = 0; t < 3 && t < tiles; ++t) transfer(t);
         look(0);
