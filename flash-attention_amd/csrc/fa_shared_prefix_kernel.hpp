@@ -9,12 +9,14 @@
 // Both products are transposed (S^T = K.Q^T; the score registers, rounded to the cache's type, are the B operand of
 // O^T += V^T.P^T), scores, maxima, sums and O are 32-bit.  P is rounded once, as every matrix product's operand must be; its
 // sum l is taken before that.  A workgroup has one of two forms: shared_few_rows (bound by reading K and V) and
-// shared_many_rows (bound by the matrix pipe and one wave's instruction issue), chosen by the number of rows.
+// shared_many_rows (matrix products; what bounds it stands there), chosen by the number of rows.
 // fa_shared_prefix_merge_kernel joins the parts.
 //
-// Measured (one MI355X, kernels alone; a large copy moves 4.9 TB/s, a large matrix product runs at 1.3 PFLOP/s):
-//   one token of each of 128 requests, 1 024 own keys each, no prefix, 8 K/V heads of 4, D = 128: 4.4 TB/s (D = 256 4.2, D = 64 3.7);
-//   one request's prompt against itself, D = 128: 950 - 1 010 TFLOP/s; against a prefix of many rows D = 256 545 - 590, D = 64 535.
+// Measured (one MI355X, kernels alone under the profiler, profiles/paged_forms.txt; 8 K/V heads of 4; a large copy moves 4.9 TB/s, a
+// large matrix product runs at 1.3 PFLOP/s), D = 64 / 128 / 256:
+//   one token of each of 128 requests, up to 1 024 own keys: 3.3 / 4.4 / 4.4 TB/s; up to 2 048: 4.2 / 4.8 / 5.1;
+//   8 prompts of up to 2 048 tokens behind 8 192 keys: 692 / 912 / 921 TFLOP/s; one of 4 096 against itself: 515 / 724 / 724;
+//   256 stacked tokens behind 16 384 keys: 364 / 564 / 552 TFLOP/s.
 //
 // Masks.  A tile that holds a masked place for some row of the wave (the end of the range, the causal diagonal, a page that
 // is none) takes the masked form of the step: scores of masked places become -inf whatever K holds there, and V is
@@ -134,7 +136,10 @@ struct SharedCfg<256> {
 };
 
 // The division of a launch into workgroups (SharedPlan), from the requests' lengths; every wave computes it for itself (no
-// barrier: all write the same numbers to LDS, each reads what it has written).
+// barrier: all write the same numbers to LDS, each reads what it has written).  That is one round of loads for every 128 requests
+// and two of lane sums for every 64, in each of about B x Hkv workgroups: nothing beside 128 requests' keys (one token each, up to 128
+// own keys, 32 heads on 8: 26 us), more than the keys from some 500 on (512: 155 us, 1 000: 444, 2 000: 1 484, 4 000: 5 459).
+
 // LDS, until the first transfer: per request its first token, its own keys, the stacked tokens and the items before it.
 struct SharedTables {
     int *tok0, *keys, *stacked, *items;
@@ -264,7 +269,7 @@ __device__ __forceinline__ int64_t part_slot(const SharedPrefixParams& p, const 
 // Up to 16 * RB rows: a single token's heads, or a few tokens'.  The work is bound by reading K and V, so each wave
 // takes a quarter of the item's keys for itself, 16 keys (a granule, on one page) at a time, through a ring of its own:
 // no barrier in the loop, and two granules and more per wave on their way (K and V through one ring of four waves with a barrier a
-// tile: 3.1 TB/s where this reaches 4.4; D = 256 1.4 and 4.2).  S^T = K.Q^T is one 16 x 16 block per 16 rows
+// tile: 3.1 TB/s where this reached 4.4; D = 256 1.4 and 4.0).  S^T = K.Q^T is one 16 x 16 block per 16 rows
 // (v_mfma 16x16x32), whose registers are the B operand of O^T += V^T.P^T (16x16x16) as they are.  The four waves' sums are joined
 // through LDS at the end.
 // Bank conflicts: a K read takes 16 rows' 16 bytes of one column, a V read 8 rows' 32 bytes (half a wave at a time); the
@@ -544,10 +549,15 @@ __device__ __forceinline__ void shared_few_rows(const SharedPrefixParams& p, con
 // Many rows: four waves of 32, key tiles of kTk keys shared through a ring of four stages (three on their way), one barrier a
 // tile.  Scores of tile t + 1 run on the matrix pipe beside the exponentials of tile t, then V^T.P^T beside the maximum of t + 1,
 // written out instruction by instruction; O lies in named accumulator registers, which the compiler neither copies nor
-// counts.  That interleaving took one prompt against itself from 760 to 913 TFLOP/s, less scalar work to 954, transfers in pairs
-// and Q's loads beside the first pages' to 1 006.  Bound by one wave's issue: 4.7 cycles an instruction, 8.7 an exponential,
-// beside 32 cycles of matrix work each.  64 rows to a wave would halve the LDS reads and the transfers; built, it ran at 940
-// (two waves to a workgroup) and needed more registers than there are where its other costs were cut.
+// counts.  That interleaving took one prompt of 4 096 tokens behind 8 192 keys (D = 128) from 760 to 913 TFLOP/s, less scalar work
+// to 954, transfers in pairs and Q's loads beside the first pages' to 1 006 (966 - 1 017 on other boxes).
+// What bounds it (counters of that prompt, profiles/paged_counters.txt): the matrix pipe is busy 48 % of the time (D = 256, 16
+// heads on 4: 45 %); of the waves' cycles 32 % (17 %) wait to issue and 22 % (28 %) for memory, LDS or the barrier.  A plain
+// instruction takes 4.7 cycles, an exponential 8.7, a matrix instruction 32, and a step of D = 128 has 69 vector instructions to 16
+// matrix ones; two waves share a SIMD at D = 64 and 128 (183 + 32 and 154 + 64 registers), one has it at D = 256.  How much of the
+// rest is the barrier of each tile, the wait between scores and V, or the masked tiles was not separated.  64 rows to a
+// wave would halve the LDS reads and the transfers; built, it ran at 940 where this ran at 979 (two waves to a workgroup), and
+// needed more registers than there are where its other costs were cut.
 template <typename E, int D>
 __device__ __forceinline__ void shared_many_rows(const SharedPrefixParams& p, const SharedItem& it, int tok, char* ring) {
     using HD = HeadDim<D>;

@@ -330,7 +330,8 @@ enum { FA_DTYPE_FP16 = 0, FA_DTYPE_BF16 = 1 };
  * among them).  A table entry outside [0, n_pages) names no page: its keys take no part.  Lengths are clamped to what the
  * table names, q_start (ascending) to [0, T].  Rows that see no key are 0; rows of dO that belong to no request keep their
  * bytes.  dO must not overlap dQ.
- *   B is at most 4000, Hq / cache->heads at most 128.  max_k_len: no request holds more own keys than this as far as the
+ *   B is at most 4000 (each workgroup reads all lengths: from some 400 requests on several calls of 256, each with its entries
+ * of q_start and k_len and its rows of the table, are faster), Hq / cache->heads at most 128.  max_k_len: no request holds more own keys than this as far as the
  * host knows (it bounds the workspace; a longer request is still computed in full).  prefix_len is a host number: a captured
  * launch keeps it.
  *   workspace: fa_shared_prefix_workspace(...) bytes, 16-byte aligned, for this call alone until it has run

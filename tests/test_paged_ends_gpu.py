@@ -139,3 +139,19 @@ def test_page_0_is_nothing_where_no_page_is_named(fa, D, dtype, bad):
         b.table[0][2 % len(b.table[0])] = 2 ** 31 - 1
         check(fa, b)
         check(fa, b, causal=False)
+
+
+def test_a_batch_in_several_calls(fa):
+    """Each call with its own entries of q_start and k_len and its own rows of the table writes its own rows of one output."""
+    b = Batch(fa, [1, 0, 3, 1, 140, 2, 1, 1, 5], [9, 4, 70, 33, 500, 2, 129, 64, 300], 333, 4, 2, 128, 16, BF16, seed=60, pad=4)
+    q_start, k_len, table, prefix = ints(b.start), ints(b.held), ints(b.table), ints(b.prefix)
+    out = torch.full_like(b.q, 3.5)
+    for lo, hi in ((4, 7), (0, 4), (7, 9)):
+        before = out.clone()
+        fa.attention_shared_prefix(b.q, b.cache, q_start[lo:hi + 1], k_len[lo:hi], table[lo:hi], prefix, 333, out=out)
+        mine = torch.zeros(b.q.shape[0], dtype=torch.bool, device=DEV)
+        mine[b.start[lo]:b.start[hi]] = True
+        assert torch.equal(out[~mine], before[~mine])
+    want, tol = b.expected()
+    n = b.start[-1]
+    assert bool(((out.double() - want).abs() <= tol)[:n].all()) and bool((out[n:] == 3.5).all())
